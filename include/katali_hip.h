@@ -46,6 +46,8 @@ extern "C" {
 #define KATALI_HIP_E_TIMEOUT (-6)     /* in-kernel dependency wait expired */
 
 #define KATALI_HIP_TYPE_F32 0u
+#define KATALI_HIP_TYPE_F16 1u        /* attention caches only */
+#define KATALI_HIP_TYPE_BF16 30u      /* attention caches only */
 #define KATALI_HIP_TYPE_Q4_K 12u
 #define KATALI_HIP_TYPE_Q6_K 14u
 
@@ -150,6 +152,111 @@ int katali_hip_add_rmsnorm(float *x_dev, const float *delta_dev, float scale, co
 int katali_hip_rmsnorm_matvec_f32(const float *x_dev, const float *delta_dev, float scale, float *x_out_dev,
                                   const float *norm_w_dev, uint64_t n, float eps, float *xn_dev,
                                   const float *w_dev, uint64_t rows, float *y_dev);
+
+/* ---- attention over key/value caches ---------------------------------------- */
+/* The steps between a layer's q/k/v projections and its o projection, for the
+ * rows of a batch: katali_hip_kv_append stores the new k and v rows, then
+ * katali_hip_attn (or katali_hip_attn_shared) attends. They stand for the
+ * engine's per-token qk-norm, rope, KV store and katali_gguf_gqa_* calls
+ * (V/src/gguf_model.c:616-663, V/src/gguf_kernels.c:115-164,247-301), which
+ * take one row, one sequence and an fp32 cache.
+ *
+ * Rows. q, out and new k/v rows are fp32, packed sequence behind sequence:
+ * row r is [n_head][head_dim] (k, v: [n_kv_head][head_dim]). Sequence s has
+ * the packed rows q_start[s] .. q_start[s+1]-1 and kv_len[s] keys, the rows'
+ * own among them: its rows are its newest positions, packed row
+ * q_start[s+1]-1 stands at position kv_len[s]-1. q_start NULL: one row per
+ * sequence, row s (n_rows == n_seq, max_q == 1). Rows before q_start[0], from
+ * q_start[n_seq] on and past a sequence's first max_q are left as they were.
+ * Caches: key j of sequence s and key head h at s * kv_seq_stride + j *
+ * kv_row_stride + h * kv_head_stride values, head_dim values on end, k and v
+ * alike; head h of q reads key head h / (n_head / n_kv_head).
+ *
+ * What a row sees: keys [0, kv_len[s]); with `causal` none behind its own
+ * position, but all before prefix_len[s] (a prefix seen from both sides);
+ * with doc_start / doc_end only keys doc_start[r] .. doc_end[r]-1 (its
+ * document, or a window). All of them hold together. A row that sees nothing
+ * gives zeros; values of keys that a row does not see, infinities and NaN
+ * among them, never reach its output (NaN or infinity in a row's q or in a
+ * visible k or v does). Device arrays are clamped to the sizes given here, so
+ * that no content of theirs is read or written out of range.
+ *
+ * Scores: x = scale * (q . k); softcap > 0: x = softcap * tanh(x / softcap);
+ * slopes: x -= slopes[h] * |position - j|. The softmax runs in fp32;
+ * products keep 22 bits of q and of the weights (fp16 caches) or all 24.
+ *
+ * Limits: head_dim 64, 128 or 256; n_head a multiple of n_kv_head, <= 1024;
+ * n_seq <= 65535; q, k, v, out 16-byte aligned, cache strides multiples of 16
+ * bytes, a row stride under 2^27 bytes; q and out do not overlap. Sums of split rows go through a library
+ * scratch (64 MB, allocated by the first call, which must be outside graph
+ * capture); calls that overlap on one GPU share it and race. */
+typedef struct KataliHipAttn {
+    uint32_t struct_size;                  /* sizeof(KataliHipAttn) */
+    uint32_t kv_type;                      /* F32, F16 or BF16: the caches' values */
+    uint32_t n_head, n_kv_head, head_dim;
+    uint32_t n_seq;                        /* sequences */
+    uint32_t n_rows;                       /* packed rows the buffers hold */
+    uint32_t max_q;                        /* the most rows of a sequence, >= 1 */
+    uint32_t max_kv;                       /* rows a cache has for each sequence */
+    uint32_t causal;
+    const int32_t *q_start;                /* device [n_seq + 1] or NULL */
+    const int32_t *kv_len;                 /* device [n_seq] */
+    uint64_t kv_seq_stride, kv_row_stride, kv_head_stride; /* in cache values */
+    float scale;
+    float softcap;                         /* 0: none */
+    const float *slopes;                   /* device [n_head] or NULL */
+    const int32_t *prefix_len;             /* device [n_seq] or NULL */
+    const int32_t *doc_start, *doc_end;    /* device [n_rows] or NULL */
+} KataliHipAttn;
+
+/* out[n_rows][n_head][head_dim] of q against the caches. */
+int katali_hip_attn(const KataliHipAttn *attn, const float *q_dev, const void *k_dev, const void *v_dev,
+                    float *out_dev);
+
+/* A prefix that every sequence of the batch shares (a common instruction or
+ * document), stored once: key j at j * row_stride + h * head_stride values,
+ * of the caches' type. Its n_prefix keys stand before each sequence's own:
+ * own key j is at position n_prefix + j, and prefix_len, doc_start and
+ * doc_end count on that axis; kv_len and max_kv count own keys alone. Where
+ * sequences have few rows the prefix is read once for the rows of all of
+ * them. n_prefix >= 1, n_prefix + max_kv < 2^31 - 4096. */
+typedef struct KataliHipAttnPrefix {
+    uint32_t struct_size;                  /* sizeof(KataliHipAttnPrefix) */
+    uint32_t n_prefix;
+    const void *k, *v;                     /* device */
+    uint64_t row_stride, head_stride;
+} KataliHipAttnPrefix;
+int katali_hip_attn_shared(const KataliHipAttn *attn, const KataliHipAttnPrefix *prefix, const float *q_dev,
+                           const void *k_dev, const void *v_dev, float *out_dev);
+
+/* KATALI_HIP_OK when katali_hip_attn (prefix NULL) or katali_hip_attn_shared
+ * takes these descriptors, else the code and last-error message the call
+ * would give for them; needs no device. */
+int katali_hip_attn_check(const KataliHipAttn *attn, const KataliHipAttnPrefix *prefix);
+
+/* The step before: each packed row's q and k heads are normed (where weights
+ * are given: x / sqrt(mean(x^2) + eps) * w over head_dim), the first n_rot
+ * values of a head turned by the row's position, q written to q_out (may be
+ * q), k and v stored in the caches at the row's own position, rounded once.
+ * Pair i (values i and i + n_rot/2, or 2i and 2i + 1 when interleaved) turns by
+ * (position + pos0) * base^(-2i / n_rot), formed in 64 bits. pos0: keys that
+ * stand before the caches' first (a shared prefix). attn's geometry, q_start,
+ * kv_len (the new rows counted) and strides apply, its masks do not; a row
+ * whose position is outside [0, max_kv) has its q written and nothing stored.
+ * Rows of two sequences that share cache memory race. n_rot even, <= head_dim, 0: no
+ * rotation; base > 0, finite. */
+typedef struct KataliHipRope {
+    uint32_t struct_size;                  /* sizeof(KataliHipRope) */
+    uint32_t n_rot;
+    uint32_t interleaved;
+    uint32_t pos0;
+    float base;
+    float eps;
+    const float *q_norm_w, *k_norm_w;      /* device [head_dim] or NULL */
+} KataliHipRope;
+int katali_hip_kv_append(const KataliHipAttn *attn, const KataliHipRope *rope, const float *q_dev,
+                         const float *k_new_dev, const float *v_new_dev, float *q_out_dev, void *k_dev,
+                         void *v_dev);
 
 /* ---- fused MoE layer (README.md:13, one GPU call per MoE layer) ----------- */
 typedef struct KataliHipMoe {

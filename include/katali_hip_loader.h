@@ -78,6 +78,16 @@ int katali_gpu_moe_route_batch(const float *logits_dev, uint32_t n_tokens, uint3
 /* The MoE layer over a batch of up to 64 tokens (batched prefill). */
 int katali_gpu_moe_batch(const KataliHipMoe *moe, const KataliHipMoeBatch *batch, const float *x_dev,
                          float *y_dev);
+/* The steps between the q/k/v and o projections: new rows into the caches,
+ * attention over them (V/src/gguf_model.c:616-663). */
+int katali_gpu_kv_append(const KataliHipAttn *attn, const KataliHipRope *rope, const float *q_dev,
+                         const float *k_new_dev, const float *v_new_dev, float *q_out_dev, void *k_dev,
+                         void *v_dev);
+int katali_gpu_attn(const KataliHipAttn *attn, const float *q_dev, const void *k_dev, const void *v_dev,
+                    float *out_dev);
+int katali_gpu_attn_shared(const KataliHipAttn *attn, const KataliHipAttnPrefix *prefix, const float *q_dev,
+                           const void *k_dev, const void *v_dev, float *out_dev);
+int katali_gpu_attn_check(const KataliHipAttn *attn, const KataliHipAttnPrefix *prefix);
 /* Pipelined uploads through a pinned ring and a copy stream (the expert
  * tier's miss path; katali_hip_stager_* in katali_hip.h). */
 int katali_gpu_stager_create(uint64_t chunk_bytes, uint32_t n_chunks, void **stager);
@@ -139,6 +149,12 @@ typedef struct KataliHipApi {
     int (*stager_mark)(void *, uint64_t *);
     int (*stager_upload)(void *, void *, const void *, uint64_t, uint64_t);
     int (*stager_fence)(void *);
+    int (*kv_append)(const KataliHipAttn *, const KataliHipRope *, const float *, const float *, const float *,
+                     float *, void *, void *);
+    int (*attn)(const KataliHipAttn *, const float *, const void *, const void *, float *);
+    int (*attn_shared)(const KataliHipAttn *, const KataliHipAttnPrefix *, const float *, const void *, const void *,
+                       float *);
+    int (*attn_check)(const KataliHipAttn *, const KataliHipAttnPrefix *);
 } KataliHipApi;
 
 /* NULL when the library could not be loaded or an entry point is missing. */

@@ -418,6 +418,124 @@ int moe_batch_impl(const KataliHipMoe *m, const KataliHipMoeBatch *b, const floa
                     "moe batch launch");
 }
 
+// Partial sums of split attention rows (ATTN_SCRATCH bytes, allocated once).
+void *g_attn = nullptr;
+
+int attn_scratch() {
+    if (g_attn) return KATALI_HIP_OK;
+    if (g_capturing) return fail(KATALI_HIP_E_INVALID, "first attention call must happen outside graph capture");
+    hipError_t e = hipMalloc(&g_attn, kq::ATTN_SCRATCH);
+    if (e == hipSuccess) return KATALI_HIP_OK;
+    g_attn = nullptr;
+    return fail(KATALI_HIP_E_NOMEM, "attention scratch: %s", hipGetErrorString(e));
+}
+
+uint32_t cache_value_bytes(uint32_t type) { return type == KATALI_HIP_TYPE_F32 ? 4 : 2; }
+
+// The rules of every attention entry (and of katali_hip_attn_check, which
+// needs no device), of the descriptors alone.
+int attn_shape(const KataliHipAttn *a, const KataliHipAttnPrefix *p) {
+    if (!a || a->struct_size < sizeof(KataliHipAttn)) return fail(KATALI_HIP_E_INVALID, "null or short attention descriptor");
+    if (a->kv_type != KATALI_HIP_TYPE_F32 && a->kv_type != KATALI_HIP_TYPE_F16 && a->kv_type != KATALI_HIP_TYPE_BF16)
+        return fail(KATALI_HIP_E_UNSUPPORTED, "cache type %u (F32=0, F16=1, BF16=30)", a->kv_type);
+    if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256)
+        return fail(KATALI_HIP_E_UNSUPPORTED, "head_dim=%u (64, 128 or 256)", a->head_dim);
+    if (!a->n_head || a->n_head > 1024 || !a->n_kv_head || a->n_head % a->n_kv_head)
+        return fail(KATALI_HIP_E_INVALID, "n_head=%u n_kv_head=%u (a multiple of n_kv_head, at most 1024)", a->n_head,
+                    a->n_kv_head);
+    if (!a->n_seq || a->n_seq > 65535) return fail(KATALI_HIP_E_INVALID, "n_seq=%u (1..65535)", a->n_seq);
+    if (!a->max_q) return fail(KATALI_HIP_E_INVALID, "max_q=0");
+    if (!a->q_start && (a->n_rows != a->n_seq || a->max_q != 1))
+        return fail(KATALI_HIP_E_INVALID, "n_rows=%u max_q=%u without q_start (one row per sequence: %u and 1)", a->n_rows,
+                    a->max_q, a->n_seq);
+    if (!a->kv_len) return fail(KATALI_HIP_E_INVALID, "null kv_len");
+    // row counts that the kernels' 32-bit grids and row indexes hold
+    const uint64_t per_seq = a->max_q < a->n_rows ? a->max_q : a->n_rows;
+    if ((uint64_t)a->n_rows * a->n_head > 0x7FFF0000ull || (uint64_t)a->n_seq * per_seq * a->n_head > 0x7FFF0000ull)
+        return fail(KATALI_HIP_E_UNSUPPORTED, "n_rows=%u n_seq=%u max_q=%u n_head=%u: above 2^31 rows x heads", a->n_rows,
+                    a->n_seq, a->max_q, a->n_head);
+    const uint64_t n_prefix = p ? p->n_prefix : 0;
+    if (n_prefix + a->max_kv >= 0x7FFFF000ull)
+        return fail(KATALI_HIP_E_UNSUPPORTED, "%llu keys above 2^31 - 4096", (unsigned long long)(n_prefix + a->max_kv));
+    const uint32_t eb = cache_value_bytes(a->kv_type), unit = 16 / eb;
+    auto strides = [&](uint64_t row, uint64_t head, uint64_t seq, const char *what) -> int {
+        if (row % unit || head % unit || seq % unit)
+            return fail(KATALI_HIP_E_INVALID, "%s strides must be multiples of %u values (16 bytes)", what, unit);
+        if (row >= (1ull << 27) / eb || head >= (1ull << 60) || seq >= (1ull << 60))
+            return fail(KATALI_HIP_E_UNSUPPORTED, "%s strides too large (a row's: under 2^27 bytes)", what);
+        return KATALI_HIP_OK;
+    };
+    int rc = strides(a->kv_row_stride, a->kv_head_stride, a->kv_seq_stride, "cache");
+    if (rc) return rc;
+    if (!isfinite(a->scale) || !isfinite(a->softcap) || a->softcap < 0.0f)
+        return fail(KATALI_HIP_E_INVALID, "scale=%g softcap=%g", (double)a->scale, (double)a->softcap);
+    if (p) {
+        if (p->struct_size < sizeof(KataliHipAttnPrefix)) return fail(KATALI_HIP_E_INVALID, "short prefix descriptor");
+        if (!p->n_prefix) return fail(KATALI_HIP_E_INVALID, "n_prefix=0");
+        if (!p->k || !p->v) return fail(KATALI_HIP_E_INVALID, "null prefix");
+        if (((uintptr_t)p->k | (uintptr_t)p->v) % 16) return fail(KATALI_HIP_E_INVALID, "prefix must be 16-byte aligned");
+        if ((rc = strides(p->row_stride, p->head_stride, 0, "prefix"))) return rc;
+    }
+    return KATALI_HIP_OK;
+}
+
+void attn_args(const KataliHipAttn *a, kq::AttnArgs &g) {
+    memset(&g, 0, sizeof g);
+    g.seq_stride = a->kv_seq_stride;
+    g.row_stride = a->kv_row_stride;
+    g.head_stride = a->kv_head_stride;
+    g.q_start = a->q_start;
+    g.kv_len = a->kv_len;
+    g.prefix_len = a->prefix_len;
+    g.doc_start = a->doc_start;
+    g.doc_end = a->doc_end;
+    g.slopes = a->slopes;
+    g.n_head = a->n_head;
+    g.n_kv = a->n_kv_head;
+    g.group = a->n_head / a->n_kv_head;
+    g.n_seq = a->n_seq;
+    g.n_rows = a->n_rows;
+    g.max_q = a->max_q < a->n_rows ? a->max_q : a->n_rows;
+    g.max_kv = a->max_kv;
+    g.causal = a->causal ? 1 : 0;
+    g.scale = a->scale;
+    g.softcap = a->softcap;
+}
+
+bool ranges_meet(const void *a, uint64_t an, const void *b, uint64_t bn) {
+    const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
+    return pa < pb + bn && pb < pa + an;
+}
+
+int attn_impl(const KataliHipAttn *a, const KataliHipAttnPrefix *p, const float *q, const void *k, const void *v,
+              float *out) {
+    int rc = attn_shape(a, p);
+    if (rc) return rc;
+    if (!a->n_rows) return ensure();
+    if (!q || !out || (a->max_kv && (!k || !v))) return fail(KATALI_HIP_E_INVALID, "null buffer");
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16)
+        return fail(KATALI_HIP_E_INVALID, "q, k, v and out must be 16-byte aligned");
+    const uint64_t row_bytes = (uint64_t)a->n_rows * a->n_head * a->head_dim * 4;
+    if (ranges_meet(q, row_bytes, out, row_bytes)) return fail(KATALI_HIP_E_INVALID, "out overlaps q");
+    if ((rc = ensure()) || (rc = attn_scratch())) return rc;
+    kq::AttnArgs g;
+    attn_args(a, g);
+    g.q = q;
+    g.k = k;
+    g.v = v;
+    g.out = out;
+    if (p) {
+        g.pk = p->k;
+        g.pv = p->v;
+        g.p_row_stride = p->row_stride;
+        g.p_head_stride = p->head_stride;
+        g.n_shared = p->n_prefix;
+    }
+    const kq::AttnPlan plan = kq::attn_plan(g.n_seq, g.n_rows, g.max_q, g.n_kv, g.group, g.max_kv, g.n_shared,
+                                            a->head_dim, (uint32_t)kq::device_cu_count());
+    return launched(kq::launch_attn(g, a->kv_type, a->head_dim, plan, g_attn, g_stream), "attention");
+}
+
 }  // namespace
 
 extern "C" {
@@ -663,6 +781,58 @@ int katali_hip_rmsnorm_matvec_f32(const float *x, const float *delta, float scal
     }
     return launched(kq::launch_norm_router(x, delta, scale, x_out, nw, n, eps, xn, w, rows, y, g_stream),
                     "rmsnorm_matvec_f32");
+}
+
+int katali_hip_attn_check(const KataliHipAttn *attn, const KataliHipAttnPrefix *prefix) {
+    return attn_shape(attn, prefix);
+}
+
+int katali_hip_attn(const KataliHipAttn *attn, const float *q, const void *k, const void *v, float *out) {
+    return attn_impl(attn, nullptr, q, k, v, out);
+}
+
+int katali_hip_attn_shared(const KataliHipAttn *attn, const KataliHipAttnPrefix *prefix, const float *q, const void *k,
+                           const void *v, float *out) {
+    if (!prefix) return fail(KATALI_HIP_E_INVALID, "null prefix descriptor");
+    return attn_impl(attn, prefix, q, k, v, out);
+}
+
+int katali_hip_kv_append(const KataliHipAttn *a, const KataliHipRope *r, const float *q, const float *k_new,
+                         const float *v_new, float *q_out, void *k, void *v) {
+    int rc = attn_shape(a, nullptr);
+    if (rc) return rc;
+    if (!r || r->struct_size < sizeof(KataliHipRope)) return fail(KATALI_HIP_E_INVALID, "null or short rope descriptor");
+    if (r->n_rot % 2 || r->n_rot > a->head_dim)
+        return fail(KATALI_HIP_E_INVALID, "n_rot=%u (even, at most head_dim %u)", r->n_rot, a->head_dim);
+    if (!(r->base > 0.0f) || !isfinite(r->base) || !isfinite(r->eps) || r->eps < 0.0f)
+        return fail(KATALI_HIP_E_INVALID, "rope base=%g eps=%g", (double)r->base, (double)r->eps);
+    if (!a->n_rows) return ensure();
+    if (!q || !k_new || !v_new || !q_out || (a->max_kv && (!k || !v))) return fail(KATALI_HIP_E_INVALID, "null buffer");
+    if (((uintptr_t)q | (uintptr_t)k_new | (uintptr_t)v_new | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v) % 16)
+        return fail(KATALI_HIP_E_INVALID, "rows and caches must be 16-byte aligned");
+    const uint64_t qb = (uint64_t)a->n_rows * a->n_head * a->head_dim * 4;
+    const uint64_t kb = (uint64_t)a->n_rows * a->n_kv_head * a->head_dim * 4;
+    if ((q != q_out && ranges_meet(q, qb, q_out, qb)) || ranges_meet(k_new, kb, q_out, qb) || ranges_meet(v_new, kb, q_out, qb))
+        return fail(KATALI_HIP_E_INVALID, "q_out overlaps an input (it may be q itself)");
+    if ((rc = ensure())) return rc;
+    kq::AttnArgs g;
+    attn_args(a, g);
+    kq::RopeArgs ra;
+    memset(&ra, 0, sizeof ra);
+    ra.q = q;
+    ra.k = k_new;
+    ra.v = v_new;
+    ra.q_out = q_out;
+    ra.k_cache = k;
+    ra.v_cache = v;
+    ra.q_w = r->q_norm_w;
+    ra.k_w = r->k_norm_w;
+    ra.eps = r->eps;
+    ra.n_rot = r->n_rot;
+    ra.interleaved = r->interleaved ? 1 : 0;
+    ra.pos0 = r->pos0;
+    ra.log2_base = log2((double)r->base);
+    return launched(kq::launch_kv_append(g, ra, a->kv_type, a->head_dim, g_stream), "kv_append");
 }
 
 int katali_hip_moe_route_batch(const float *logits, uint32_t n_tokens, uint32_t n_expert, int32_t n_sel,

@@ -1,0 +1,726 @@
+// kq_attn.hip — softmax attention of query rows over their sequences' caches,
+// and over a prefix that all sequences share.
+//
+//   x_j = scale (q . k_j);  x_j = cap tanh(x_j / cap) with a cap;
+//   x_j -= slope_h |pos - j| with slopes;  o = sum_j p_j v_j, p = softmax over
+//   the row's keys [lo, hi), where lo and hi come from the causal rule, the
+//   two-sided prefix and the row's document. A row with no key gives zeros.
+//
+// One pass over the keys with a running maximum and sum (in log2 units). q
+// and the outputs are fp32, and the matrix instructions take 16-bit operands
+// with 16-bit caches, so q and p are each split into 16-bit terms, two of fp16
+// (22 bits together) or three of bf16 (24), and each product is formed once per
+// term into the same fp32 accumulators: nothing is rounded to 16 bits. With
+// fp32 caches the fp32 matrix instructions are used.
+//
+// k_attn: a wave takes 16 rows (query rows x the heads of one key head), one
+// row per lane column of the matrix tile, and walks its keys in tiles of 32
+// (16 with fp32 caches). It computes S^T = K Q^T, so that a lane holds scores
+// of one row only and row maxima need two cross-lane steps, and O^T = V^T P^T,
+// whose B operand is P^T in the very registers that S^T came in: the keys of
+// an operand may stand in any order if both operands have the same. V^T's
+// operand wants four keys of one column in a lane; a lane loads 4 rows of V,
+// D/16 columns each, and exchanges halves between them (v_perm), no LDS. The
+// four waves of a workgroup share 16 rows and take every fourth tile (few
+// rows: the keys are what there is to spread), or take 64 rows.
+#include <type_traits>
+
+#include "kq_attn.h"
+
+namespace kq {
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.44269504088896341f;
+constexpr float NEG_INF = -__builtin_inff();
+
+template <class T, class S>
+__device__ __forceinline__ T bits(const S &s) {
+    static_assert(sizeof(T) == sizeof(S), "bits: sizes differ");
+    T t;
+    __builtin_memcpy(&t, &s, sizeof(T));
+    return t;
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// max / sum over the four lanes (one per 16-lane row) that hold one query row
+__device__ __forceinline__ float rows_max(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float rows_sum(float v) {
+    v = swap_sum<16>(v, v);
+    return swap_sum<32>(v, v);
+}
+
+// tanh to about 1e-7 of its value: below 1 the continued fraction
+// u / (1 + u^2 / (3 + u^2 / (5 + u^2 / (7 + u^2 / 9)))), above it
+// 1 - 2 / (e^2u + 1), both over one reciprocal. NaN stays NaN.
+__device__ __forceinline__ float tanh_fast(float u) {
+    const float u2 = u * u;
+    const bool small = fabsf(u) < 1.0f;
+    const float num = u * fmaf(u2, u2 + 105.0f, 945.0f);
+    const float t = exp2_hw(u * (2.0f * LOG2E));
+    const float den = small ? fmaf(u2, fmaf(u2, 15.0f, 420.0f), 945.0f) : t + 1.0f;
+    const float r = __builtin_amdgcn_rcpf(den);
+    return small ? num * r : fmaf(-2.0f, r, 1.0f);
+}
+
+// Two fp32 values as 16-bit terms each, every term packed: the first takes the
+// leading bits of a value, the next the leading bits of what is left. fp16 cut
+// toward zero (one instruction for both values) keeps 11 bits a term, 22 in
+// two; bf16 keeps 8 (cut by taking the upper half words), all 24 in three.
+template <int TY>
+constexpr int TERMS = TY == ATTN_F32 ? 1 : TY == ATTN_F16 ? 2 : 3;
+template <int TY>
+__device__ __forceinline__ void split(float x, float y, uint32_t (&w)[TERMS<TY>]) {
+    if constexpr (TY == ATTN_F16) {
+        const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+        w[0] = bits<uint32_t>(h);
+        w[1] = bits<uint32_t>(__builtin_amdgcn_cvt_pkrtz(x - (float)h[0], y - (float)h[1]));
+    } else {
+#pragma unroll
+        for (int n = 0; n < 3; n++) {
+            w[n] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+            x -= __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+            y -= __uint_as_float(__float_as_uint(y) & 0xFFFF0000u);
+        }
+    }
+}
+
+template <int TY>
+__device__ __forceinline__ f32x4 mfma32(const uint4 &a, const uint4 &b, f32x4 c) {
+    if constexpr (TY == ATTN_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(bits<f16x8>(a), bits<f16x8>(b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bits<b16x8>(a), bits<b16x8>(b), c, 0, 0, 0);
+}
+
+// One value of a cache row as fp32.
+template <int TY>
+__device__ __forceinline__ float ld_kv(const void *p, uint64_t i) {
+    if constexpr (TY == ATTN_F32) return ((const float *)p)[i];
+    else if constexpr (TY == ATTN_F16) return (float)((const _Float16 *)p)[i];
+    else return __uint_as_float((uint32_t)((const uint16_t *)p)[i] << 16);
+}
+
+// A row's score of one key in log2 units, from the accumulated product s.
+struct Score {
+    float mul;     // product -> score (with a cap: -> score / cap)
+    float cap;     // cap log2(e), 0 for none
+    float slope;   // slope log2(e)
+};
+__device__ __forceinline__ float score(const Score &c, float s, int32_t pos, int32_t j) {
+    float y = s * c.mul;
+    if (c.cap != 0.0f) y = c.cap * tanh_fast(y);
+    if (c.slope != 0.0f) y = fmaf(-c.slope, fabsf((float)(pos - j)), y);
+    return y;
+}
+
+// What a wave's lane knows about the query row it holds (lanes 16 apart hold
+// the same row).
+struct Row {
+    int32_t row, pos, lo, hi;   // packed row, position, its keys [lo, hi)
+    uint32_t head;
+    bool valid;
+};
+
+__device__ __forceinline__ Row make_row(const AttnArgs &a, uint32_t kvh, uint32_t packed, bool pooled, uint32_t s,
+                                        const SeqRows &sr, int32_t n_row) {
+    Row r;
+    const int32_t t = (int32_t)(packed / a.group);
+    r.head = kvh * a.group + packed % a.group;
+    r.row = sr.first + t;
+    r.valid = t < n_row;
+    r.pos = r.lo = r.hi = 0;
+    if (r.valid) {
+        SeqRows own = sr;
+        if (pooled) {
+            s = seq_of_row(a, r.row);
+            own = seq_rows(a, s);
+            r.valid = r.row >= own.first && r.row < own.last && r.row - own.first < (int32_t)a.max_q;
+        }
+        r.pos = row_pos(a, own, r.row);
+        r.hi = (int32_t)a.n_shared + own.len;
+        if (a.causal) {
+            int32_t upto = r.pos + 1;
+            if (a.prefix_len) upto = max(upto, a.prefix_len[s]);
+            r.hi = min(r.hi, upto);
+        }
+        if (a.doc_start) r.lo = max(r.lo, a.doc_start[r.row]);
+        if (a.doc_end) r.hi = min(r.hi, a.doc_end[r.row]);
+        if (!r.valid) r.lo = r.hi = 0;
+    }
+    return r;
+}
+
+// min / max over the wave of an integer that 16-lane rows hold alike
+__device__ __forceinline__ int32_t row16_min(int32_t v) {
+    v = min(v, dpp_i<DPP_XOR1>(v));
+    v = min(v, dpp_i<DPP_XOR2>(v));
+    v = min(v, dpp_i<DPP_HALF_MIRROR>(v));
+    return min(v, dpp_i<DPP_MIRROR>(v));
+}
+
+template <int TY, int D>
+struct Tile {
+    static constexpr int KT = TY == ATTN_F32 ? 16 : 32;          // keys per tile
+    static constexpr int DPL = D / 16;                           // columns of V per lane
+    static constexpr int EB = TY == ATTN_F32 ? 4 : 2;            // bytes per cache value
+    static constexpr int KC = TY == ATTN_F32 ? D / 16 : D / 32;  // 16-byte pieces of a key row per lane
+    static constexpr int KR = KT / 16;                           // key rows per lane
+    static constexpr int VR = KT / 4;                            // value rows per lane
+    static constexpr int VW = DPL * EB / 4;                      // dwords of a value row per lane
+};
+
+// The keys and values of one tile in registers. K: lane l holds of key rows
+// l % 16 (+ 16) the pieces 8 (l / 16) + 32 c (fp32: 4 (l / 16) + 16 c). V: of
+// rows 4 (l / 16) + r (+ 16) the columns DPL (l % 16) ...
+template <int TY, int D>
+struct Frag {
+    using G = Tile<TY, D>;
+    uint4 k[G::KR][G::KC];
+    uint32_t v[G::VR][G::VW];
+
+    // rows j0 ..; rows from `end` on repeat the last one before it: their
+    // scores are masked, their values weigh zero and are some row's own
+    __device__ __forceinline__ void load(const char *kb, const char *vb, uint32_t row_bytes, int32_t j0, int32_t end,
+                                         int lane) {
+        const uint32_t c = lane & 15, g = lane >> 4;
+        const uint64_t at = (uint64_t)(uint32_t)j0 * row_bytes;
+        const char *kp = kb + at, *vp = vb + at;
+        const int32_t n = end - j0;
+        if (n >= G::KT) {
+            const uint32_t ko = c * row_bytes + g * 16, vo = 4 * g * row_bytes + c * (G::DPL * G::EB);
+#pragma unroll
+            for (int t = 0; t < G::KR; t++)
+#pragma unroll
+                for (int i = 0; i < G::KC; i++)
+                    k[t][i] = *(const uint4 *)(kp + (uint64_t)t * 16 * row_bytes + ko + i * 64);
+#pragma unroll
+            for (int r = 0; r < G::VR; r++) ldv(r, vp + (uint64_t)((r & 3) + (r >> 2) * 16) * row_bytes + vo);
+        } else {
+#pragma unroll
+            for (int t = 0; t < G::KR; t++) {
+                const uint32_t ko = (uint32_t)min((int32_t)c + 16 * t, n - 1) * row_bytes + g * 16;
+#pragma unroll
+                for (int i = 0; i < G::KC; i++) k[t][i] = *(const uint4 *)(kp + ko + i * 64);
+            }
+#pragma unroll
+            for (int r = 0; r < G::VR; r++)
+                ldv(r, vp + (uint32_t)min((int32_t)(4 * g) + (r & 3) + (r >> 2) * 16, n - 1) * row_bytes +
+                           c * (G::DPL * G::EB));
+        }
+    }
+    __device__ __forceinline__ void ldv(int r, const char *p) {
+        if constexpr (G::VW >= 4) {
+#pragma unroll
+            for (int w = 0; w < G::VW; w += 4) {
+                const uint4 x = *(const uint4 *)(p + 4 * w);
+                v[r][w] = x.x, v[r][w + 1] = x.y, v[r][w + 2] = x.z, v[r][w + 3] = x.w;
+            }
+        } else {
+            const uint2 x = *(const uint2 *)p;
+            v[r][0] = x.x, v[r][1] = x.y;
+        }
+    }
+};
+
+// A wave's running state over its 16 rows.
+template <int TY, int D>
+struct Wave16 {
+    using G = Tile<TY, D>;
+    static constexpr int NT = TERMS<TY>;
+    uint4 q[NT][G::KC];   // query operand: fp32 pieces, or the 16-bit terms of each value
+    Score sc;
+    float m, l;
+    f32x4 o[G::DPL];   // o[t][r]: column DPL (4 (l / 16) + r) + t of row l % 16
+
+    __device__ __forceinline__ void init(const AttnArgs &a, const Row &r, int lane) {
+        const uint32_t g = lane >> 4;
+        const float *qp = a.q + ((uint64_t)(uint32_t)r.row * a.n_head + r.head) * D;
+        constexpr int E = TY == ATTN_F32 ? 4 : 8;   // values per piece
+        float v[G::KC][E];
+        float top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < G::KC; c++)
+#pragma unroll
+            for (int i = 0; i < E; i += 4) {
+                float4 x = make_float4(0, 0, 0, 0);
+                if (r.valid) x = *(const float4 *)(qp + c * (TY == ATTN_F32 ? 16 : 32) + g * E + i);
+                v[c][i] = x.x, v[c][i + 1] = x.y, v[c][i + 2] = x.z, v[c][i + 3] = x.w;
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+            }
+        float mul = a.scale;
+        if constexpr (TY == ATTN_F32) {
+#pragma unroll
+            for (int c = 0; c < G::KC; c++)
+                q[0][c] = make_uint4(__float_as_uint(v[c][0]), __float_as_uint(v[c][1]), __float_as_uint(v[c][2]),
+                                     __float_as_uint(v[c][3]));
+        } else {
+            // fp16 terms: the row is brought to 2^12 by a power of two, so
+            // that neither a large q overflows nor a small one loses bits
+            float up = 1.0f;
+            if constexpr (TY == ATTN_F16) {
+                top = rows_max(top);
+                int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+                e = min(max(e, -100), 100);
+                up = __uint_as_float((uint32_t)(127 + 12 - e) << 23);
+                mul = a.scale * __uint_as_float((uint32_t)(127 - 12 + e) << 23);
+            }
+#pragma unroll
+            for (int c = 0; c < G::KC; c++) {
+                uint32_t w[4][NT];
+#pragma unroll
+                for (int i = 0; i < 4; i++) split<TY>(v[c][2 * i] * up, v[c][2 * i + 1] * up, w[i]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) q[n][c] = make_uint4(w[0][n], w[1][n], w[2][n], w[3][n]);
+            }
+        }
+        sc.cap = a.softcap * LOG2E;
+        sc.mul = a.softcap != 0.0f ? mul / a.softcap : mul * LOG2E;
+        sc.slope = a.slopes && r.valid ? a.slopes[r.head] * LOG2E : 0.0f;
+        m = NEG_INF;
+        l = 0.0f;
+#pragma unroll
+        for (int t = 0; t < G::DPL; t++) o[t] = f32x4{0, 0, 0, 0};
+    }
+
+    // keys j0 .. j0 + KT of one tile, those from `end` on not of its segment;
+    // whole: every row sees all of them
+    __device__ __forceinline__ void step(const Frag<TY, D> &f, const Row &row, int32_t j0, int32_t end, bool whole,
+                                         int lane) {
+        const int32_t g4 = 4 * (lane >> 4);
+        float y[G::VR];
+#pragma unroll
+        for (int t = 0; t < G::KR; t++) {
+            f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < G::KC; c++) {
+                if constexpr (TY == ATTN_F32) {
+                    const f32x4 kv = bits<f32x4>(f.k[t][c]), qv = bits<f32x4>(q[0][c]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[i], qv[i], s, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) s = mfma32<TY>(f.k[t][c], q[n][c], s);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[4 * t + r] = score(sc, s[r], row.pos, j0 + 16 * t + g4 + r);
+        }
+        if (!whole) {
+            const int32_t hi = min(row.hi, end);
+#pragma unroll
+            for (int r = 0; r < G::VR; r++) {
+                const int32_t j = j0 + (r >> 2) * 16 + g4 + (r & 3);
+                if (j < row.lo || j >= hi) y[r] = NEG_INF;
+            }
+        }
+        float top = y[0];
+#pragma unroll
+        for (int r = 1; r < G::VR; r++) top = fmaxf(top, y[r]);
+        top = rows_max(top);
+        // the maximum that scales the sums moves only when it falls behind by
+        // 2^8: most tiles then leave the accumulators alone
+        if (__any(top > m + 8.0f)) {
+            const float mn = fmaxf(m, top);
+            const float f0 = m == NEG_INF ? 0.0f : exp2_hw(m - mn);
+            m = mn;
+            l *= f0;
+#pragma unroll
+            for (int t = 0; t < G::DPL; t++) o[t] *= f0;
+        }
+        // fp16 terms of p stand 2^7 higher, so that the second ones stay normal
+        const float base = (m == NEG_INF ? 0.0f : m) - (TY == ATTN_F16 ? 7.0f : 0.0f);
+        float p[G::VR];
+#pragma unroll
+        for (int r = 0; r < G::VR; r++) {
+            p[r] = exp2_hw(y[r] - base);
+            l += p[r];
+        }
+        if constexpr (TY == ATTN_F32) {
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int t = 0; t < G::DPL; t++)
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.v[r][t]), p[r], o[t], 0, 0, 0);
+        } else {
+            uint32_t pt[4][NT];
+#pragma unroll
+            for (int i = 0; i < 4; i++) split<TY>(p[2 * i], p[2 * i + 1], pt[i]);
+#pragma unroll
+            for (int t = 0; t < G::DPL; t++) {
+                const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    w[i] = __builtin_amdgcn_perm(f.v[2 * i + 1][t / 2], f.v[2 * i][t / 2], sel);
+                const uint4 vt = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+                    o[t] = mfma32<TY>(vt, make_uint4(pt[0][n], pt[1][n], pt[2][n], pt[3][n]), o[t]);
+            }
+        }
+    }
+
+    // Whether an accumulator of the lane's row is not finite.
+    __device__ __forceinline__ bool odd() const {
+        float z = l * 0.0f;
+#pragma unroll
+        for (int t = 0; t < G::DPL; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) z = fmaf(o[t][r], 0.0f, z);
+        return !(z == 0.0f);
+    }
+};
+
+// Keys [c0, c1) of one segment: the shared prefix or a sequence's own cache.
+struct Segment {
+    const char *k, *v;    // of key c0's axis origin: key j at (j - origin) rows
+    int32_t origin, c0, c1;
+    uint32_t row_bytes;
+};
+
+__device__ __forceinline__ Segment segment(const AttnArgs &a, uint32_t eb, uint32_t kvh, uint32_t s, bool shared,
+                                           int32_t c0, int32_t c1) {
+    Segment g;
+    if (shared) {
+        const uint64_t at = (uint64_t)kvh * a.p_head_stride * eb;
+        g.k = (const char *)a.pk + at;
+        g.v = (const char *)a.pv + at;
+        g.row_bytes = (uint32_t)a.p_row_stride * eb;
+        g.origin = 0;
+        g.c0 = c0;
+        g.c1 = min(c1, (int32_t)a.n_shared);
+    } else {
+        const uint64_t at = ((uint64_t)s * a.seq_stride + (uint64_t)kvh * a.head_stride) * eb;
+        g.k = (const char *)a.k + at;
+        g.v = (const char *)a.v + at;
+        g.row_bytes = (uint32_t)a.row_stride * eb;
+        g.origin = (int32_t)a.n_shared;
+        g.c0 = max(c0, (int32_t)a.n_shared);
+        g.c1 = c1;
+    }
+    return g;
+}
+
+// A row whose accumulators are not finite, again key by key, so that values
+// only of its own keys reach it: in a matrix tile a masked key's infinity or
+// NaN meets a zero weight and spoils the rows that do not see it. One wave;
+// lane l sums columns l, l + 64, ... (out) over the keys of its own tiles.
+template <int TY, int D, int W>
+__device__ __forceinline__ void row_again(const AttnArgs &a, uint32_t kvh, uint32_t s, const Row &r, int32_t c0,
+                                          int32_t c1, int wave, int lane, float (&acc)[D / 64], float &m, float &l) {
+    using G = Tile<TY, D>;
+    const float *qp = a.q + ((uint64_t)(uint32_t)r.row * a.n_head + r.head) * D;
+    Score sc;
+    sc.cap = a.softcap * LOG2E;
+    sc.mul = a.softcap != 0.0f ? a.scale / a.softcap : a.scale * LOG2E;
+    sc.slope = a.slopes ? a.slopes[r.head] * LOG2E : 0.0f;
+    m = NEG_INF;
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 64; e++) acc[e] = 0.0f;
+    for (int sg = 0; sg < 2; sg++) {
+        const Segment g = segment(a, G::EB, kvh, s, sg == 0, c0, c1);
+        for (int32_t j0 = g.c0 + wave * G::KT; j0 < g.c1; j0 += W * G::KT)
+            for (int32_t j = max(j0, r.lo); j < min(min(j0 + G::KT, g.c1), r.hi); j++) {
+                const uint64_t at = (uint64_t)(uint32_t)(j - g.origin) * g.row_bytes;
+                float d = 0.0f;
+#pragma unroll
+                for (int e = 0; e < D / 64; e++)
+                    d = fmaf(qp[lane + 64 * e], ld_kv<TY>(g.k + at, lane + 64 * e), d);
+                const float y = score(sc, group_sum<64>(d), r.pos, j);
+                const float mn = y > m ? y : m;
+                const float f0 = m == NEG_INF ? 0.0f : exp2_hw(m - mn);
+                const float p = exp2_hw(y - (mn == NEG_INF ? 0.0f : mn));
+                l = l * f0 + p;
+#pragma unroll
+                for (int e = 0; e < D / 64; e++) acc[e] = fmaf(p, ld_kv<TY>(g.v + at, lane + 64 * e), acc[e] * f0);
+                m = mn;
+            }
+    }
+    if constexpr (TY == ATTN_F16) {   // as the tiles' sums stand
+        l *= 128.0f;
+#pragma unroll
+        for (int e = 0; e < D / 64; e++) acc[e] *= 128.0f;
+    }
+}
+
+// The item of a workgroup: which rows over which keys, and where the result goes.
+struct Item {
+    uint32_t kvh, split, tile, seq;
+    bool pooled;
+};
+__device__ __forceinline__ Item make_item(const AttnArgs &a, uint32_t id) {
+    Item it;
+    it.pooled = id >= a.own_items;
+    if (it.pooled) id -= a.own_items;
+    const uint32_t splits = it.pooled ? a.shared_splits : a.own_splits;
+    const uint32_t tiles = it.pooled ? a.shared_tiles : a.own_tiles;
+    it.kvh = id % a.n_kv;
+    id /= a.n_kv;
+    it.split = id % splits;
+    id /= splits;
+    it.tile = tiles - 1 - id % tiles;   // later rows see more keys: they start first
+    it.seq = id / tiles;
+    return it;
+}
+
+// A row's result: the output itself, or one of the partial sums that k_attn_join joins.
+__device__ __forceinline__ uint64_t row_head(const AttnArgs &a, const Row &r) {
+    return (uint64_t)(uint32_t)r.row * a.n_head + r.head;
+}
+__device__ __forceinline__ uint64_t slot_of(const AttnArgs &a, uint64_t rh, const Item &it) {
+    return rh * a.slots + (it.pooled ? a.own_splits : 0) + it.split;
+}
+
+// RS: the four waves take four row tiles and all keys of the item; else one
+// row tile and every fourth key tile.
+template <int TY, int D, bool RS>
+__global__ void __launch_bounds__(256, D <= (TY == ATTN_BF16 ? 64 : 128) ? 2 : 1) k_attn(const AttnArgs a) {
+    using G = Tile<TY, D>;
+    constexpr int W = 4;
+    __shared__ float lds_o[RS ? 1 : W][RS ? 1 : 16][RS ? 1 : D + 4];
+    __shared__ float lds_m[W][16], lds_l[W][16];
+    __shared__ float lds_row[W][D];
+    __shared__ uint64_t lds_at[16];   // packed row x head of each tile row, ~0 for none
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Item it = make_item(a, blockIdx.x);
+
+    SeqRows sr;
+    int32_t n_row;
+    if (it.pooled) {
+        sr.first = a.q_start ? min(max(a.q_start[0], 0), (int32_t)a.n_rows) : 0;
+        sr.last = a.q_start ? min(max(a.q_start[a.n_seq], sr.first), (int32_t)a.n_rows) : (int32_t)a.n_rows;
+        sr.len = 0;
+        n_row = sr.last - sr.first;
+    } else {
+        sr = seq_rows(a, it.seq);
+        n_row = min(sr.last - sr.first, (int32_t)a.max_q);
+    }
+    const uint32_t first = (it.tile * (RS ? W : 1) + (RS ? wave : 0)) * 16;
+    const Row row = make_row(a, it.kvh, first + (lane & 15), it.pooled, it.seq, sr, n_row);
+
+    // the keys any row of the tile sees, of those this item is for, and this split's share of them
+    int32_t kb = 0, ke = (int32_t)a.n_shared + sr.len;
+    if (it.pooled) ke = (int32_t)a.n_shared;
+    else if (a.shared_splits) kb = (int32_t)a.n_shared;
+    const int32_t rl = max(row.lo, kb), rh = min(row.hi, ke);
+    const bool some = rl < rh;
+    const int32_t tl = __builtin_amdgcn_readfirstlane(row16_min(some ? rl : INT32_MAX));
+    const int32_t th = __builtin_amdgcn_readfirstlane(-row16_min(some ? -rh : 0));
+    // keys that every row sees: tiles inside need no mask
+    const int32_t al = __builtin_amdgcn_readfirstlane(-row16_min(row.valid ? -row.lo : 0));
+    const int32_t ah = __builtin_amdgcn_readfirstlane(row16_min(row.valid ? row.hi : INT32_MAX));
+    int32_t c0 = 0, c1 = 0;
+    if (th > tl) {
+        const uint32_t n = (uint32_t)(th - tl), splits = it.pooled ? a.shared_splits : a.own_splits;
+        const uint32_t used = min(max((n + a.min_chunk - 1) / a.min_chunk, 1u), splits);
+        const uint32_t chunk = ((n + used - 1) / used + G::KT - 1) / G::KT * G::KT;
+        const uint64_t b = (uint64_t)it.split * chunk;
+        if (b < n) {
+            c0 = tl + (int32_t)b;
+            c1 = tl + (int32_t)min((uint64_t)n, b + chunk);
+        }
+    }
+
+    Wave16<TY, D> st;
+    st.init(a, row, lane);
+    for (int sg = 0; sg < 2; sg++) {
+        const Segment g = segment(a, G::EB, it.kvh, it.seq, sg == 0, c0, c1);
+        const int32_t step = (RS ? 1 : W) * G::KT;
+        int32_t j = g.c0 + (RS ? 0 : wave * G::KT);
+        if (j >= g.c1) continue;
+        Frag<TY, D> f;
+        f.load(g.k, g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
+        while (true) {
+            const int32_t jn = j + step;
+            const bool whole = j >= al && j + G::KT <= min(ah, g.c1);
+            if constexpr (D <= 128) {
+                Frag<TY, D> fn;
+                if (jn < g.c1) fn.load(g.k, g.v, g.row_bytes, jn - g.origin, g.c1 - g.origin, lane);
+                st.step(f, row, j, g.c1, whole, lane);
+                f = fn;
+            } else {
+                st.step(f, row, j, g.c1, whole, lane);
+                if (jn < g.c1) f.load(g.k, g.v, g.row_bytes, jn - g.origin, g.c1 - g.origin, lane);
+            }
+            j = jn;
+            if (j >= g.c1) break;
+        }
+    }
+    st.l = rows_sum(st.l);
+
+    // rows that met an infinity or NaN, key by key
+    uint64_t odd = __ballot(st.odd());
+    odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xFFFF;
+    while (odd) {
+        const int i = __builtin_ctzll(odd);
+        odd &= odd - 1;
+        Row r;
+        r.row = __builtin_amdgcn_readlane(row.row, i);
+        r.pos = __builtin_amdgcn_readlane(row.pos, i);
+        r.lo = __builtin_amdgcn_readlane(row.lo, i);
+        r.hi = __builtin_amdgcn_readlane(row.hi, i);
+        r.head = (uint32_t)__builtin_amdgcn_readlane((int)row.head, i);
+        r.valid = true;
+        float acc[D / 64], m, l;
+        row_again<TY, D, RS ? 1 : W>(a, it.kvh, it.seq, r, c0, c1, RS ? 0 : wave, lane, acc, m, l);
+#pragma unroll
+        for (int e = 0; e < D / 64; e++) lds_row[wave][lane + 64 * e] = acc[e];
+        __builtin_amdgcn_wave_barrier();
+        if ((lane & 15) == i) {
+            st.m = m;
+            st.l = l;
+#pragma unroll
+            for (int t = 0; t < G::DPL; t++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) st.o[t][q] = lds_row[wave][G::DPL * (4 * (lane >> 4) + q) + t];
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    if constexpr (RS) {
+        if (!row.valid) return;
+        float *dst;
+        float f0 = 1.0f;
+        if (a.slots) {
+            const uint64_t at = slot_of(a, row_head(a, row), it);
+            if (lane < 16) a.ml[at] = make_float2(st.m, st.l);
+            dst = a.acc + at * D;
+            if (st.l == 0.0f) return;
+        } else {
+            f0 = st.l == 0.0f ? 0.0f : 1.0f / st.l;
+            dst = a.out + row_head(a, row) * D;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int t = 0; t < G::DPL; t += 4)
+                *(float4 *)(dst + G::DPL * (4 * (lane >> 4) + q) + t) =
+                    make_float4(st.o[t][q] * f0, st.o[t + 1][q] * f0, st.o[t + 2][q] * f0, st.o[t + 3][q] * f0);
+    } else {
+        // the four waves' sums of the same rows, joined in LDS
+        if (lane < 16) {
+            lds_m[wave][lane] = st.m;
+            lds_l[wave][lane] = st.l;
+            if (wave == 0) lds_at[lane] = row.valid ? row_head(a, row) : ~0ull;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int t = 0; t < G::DPL; t += 4)
+                *(float4 *)&lds_o[wave][lane & 15][G::DPL * (4 * (lane >> 4) + q) + t] =
+                    make_float4(st.o[t][q], st.o[t + 1][q], st.o[t + 2][q], st.o[t + 3][q]);
+        __syncthreads();
+        // thread: row tid / 16, columns D/16 (tid % 16) ...
+        const int i = threadIdx.x >> 4;
+        const uint64_t rh = lds_at[i];
+        if (rh == ~0ull) return;
+        float m = NEG_INF, l = 0.0f, w[W];
+#pragma unroll
+        for (int k = 0; k < W; k++) m = fmaxf(m, lds_m[k][i]);
+#pragma unroll
+        for (int k = 0; k < W; k++) {
+            w[k] = lds_l[k][i] == 0.0f ? 0.0f : exp2_hw(lds_m[k][i] - m);
+            l += lds_l[k][i] * w[k];
+        }
+        float *dst;
+        float f0 = 1.0f;
+        if (a.slots) {
+            const uint64_t at = slot_of(a, rh, it);
+            if ((threadIdx.x & 15) == 0) a.ml[at] = make_float2(m, l);
+            if (l == 0.0f) return;
+            dst = a.acc + at * D;
+        } else {
+            f0 = l == 0.0f ? 0.0f : 1.0f / l;
+            dst = a.out + rh * D;
+        }
+#pragma unroll
+        for (int t = 0; t < G::DPL; t += 4) {
+            const int col = (threadIdx.x & 15) * G::DPL + t;
+            float x[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < W; k++) {
+                if (w[k] == 0.0f) continue;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = fmaf(lds_o[k][i][col + e], w[k], x[e]);
+            }
+            *(float4 *)(dst + col) = make_float4(x[0] * f0, x[1] * f0, x[2] * f0, x[3] * f0);
+        }
+    }
+}
+
+// The partial sums of a row, joined: one wave per (row, head).
+template <int D>
+__global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t heads4 = (a.n_head + 3) / 4;
+    const uint32_t head = blockIdx.x % heads4 * 4 + (threadIdx.x >> 6);
+    const uint32_t id = blockIdx.x / heads4, seq = id / a.max_q, t = id % a.max_q;
+    const SeqRows sr = seq_rows(a, seq);
+    if (head >= a.n_head || (int32_t)t >= sr.last - sr.first) return;
+    const uint64_t rh = (uint64_t)(uint32_t)(sr.first + (int32_t)t) * a.n_head + head;
+    float2 ml = make_float2(NEG_INF, 0.0f);
+    if ((uint32_t)lane < a.slots) ml = a.ml[rh * a.slots + lane];
+    float m = ml.x;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float w = ml.y == 0.0f ? 0.0f : exp2_hw(ml.x - m);
+    const float l = group_sum<64>(ml.y * w);
+    const float f0 = l == 0.0f ? 0.0f : 1.0f / l;
+    float x[D / 64];
+#pragma unroll
+    for (int e = 0; e < D / 64; e++) x[e] = 0.0f;
+    for (uint32_t k = 0; k < a.slots; k++) {
+        const float wk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), k));
+        if (wk == 0.0f) continue;
+        const float *p = a.acc + (rh * a.slots + k) * D;
+#pragma unroll
+        for (int e = 0; e < D / 64; e++) x[e] = fmaf(p[lane + 64 * e], wk, x[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < D / 64; e++) a.out[rh * D + lane + 64 * e] = x[e] * f0;
+}
+
+template <int TY, int D>
+static hipError_t attn_run(const AttnArgs &a, bool rows, uint32_t items, hipStream_t s) {
+    if (rows) hipLaunchKernelGGL((k_attn<TY, D, true>), dim3(items), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_attn<TY, D, false>), dim3(items), dim3(256), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !a.slots) return e;
+    hipLaunchKernelGGL((k_attn_join<D>), dim3(a.n_seq * a.max_q * ((a.n_head + 3) / 4)), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_attn(AttnArgs a, uint32_t type, uint32_t head_dim, const AttnPlan &p, void *scratch, hipStream_t s) {
+    a.own_tiles = p.own_tiles;
+    a.own_splits = p.own_splits;
+    a.shared_tiles = p.shared_tiles;
+    a.shared_splits = p.shared_splits;
+    a.slots = p.slots;
+    a.own_items = p.own_items;
+    a.min_chunk = p.min_chunk;
+    a.acc = (float *)scratch;
+    a.ml = (float2 *)((char *)scratch + (uint64_t)a.n_rows * a.n_head * p.slots * head_dim * 4);
+    const uint32_t items = p.own_items + p.shared_items;
+    auto go = [&](auto ty) -> hipError_t {
+        constexpr int TY = decltype(ty)::value;
+        if (head_dim == 64) return attn_run<TY, 64>(a, p.rows, items, s);
+        if (head_dim == 128) return attn_run<TY, 128>(a, p.rows, items, s);
+        return attn_run<TY, 256>(a, p.rows, items, s);
+    };
+    if (type == ATTN_F32) return go(std::integral_constant<int, ATTN_F32>());
+    if (type == ATTN_F16) return go(std::integral_constant<int, ATTN_F16>());
+    return go(std::integral_constant<int, ATTN_BF16>());
+}
+
+}  // namespace kq

@@ -294,4 +294,35 @@ hipError_t launch_moe_batch(const MoeArgs &a, uint32_t T, uint32_t min_big, cons
                             int32_t *meta, hipStream_t s, hipStream_t aux, hipEvent_t fork, hipEvent_t join);
 uint64_t moe_route_words();
 
+// Attention over caches (kq_attn.hip) and the step that stores new rows
+// (kq_kv.hip). Strides in cache values; arrays as KataliHipAttn describes them.
+constexpr int ATTN_F32 = 0, ATTN_F16 = 1, ATTN_BF16 = 30;   // cache types (ggml ids)
+struct AttnArgs {
+    const float *q;
+    float *out;
+    const void *k, *v, *pk, *pv;
+    uint64_t seq_stride, row_stride, head_stride, p_row_stride, p_head_stride;
+    const int32_t *q_start, *kv_len, *prefix_len, *doc_start, *doc_end;
+    const float *slopes;
+    uint32_t n_head, n_kv, group, n_seq, n_rows, max_q, max_kv, n_shared;
+    uint32_t causal;
+    float scale, softcap;
+    // the plan, set by launch_attn
+    uint32_t own_tiles, own_splits, shared_tiles, shared_splits, slots, own_items, min_chunk;
+    float *acc;
+    float2 *ml;
+};
+hipError_t launch_attn(AttnArgs a, uint32_t type, uint32_t head_dim, const AttnPlan &p, void *scratch, hipStream_t s);
+
+struct RopeArgs {
+    const float *q, *k, *v;      // new rows, packed
+    float *q_out;
+    void *k_cache, *v_cache;
+    const float *q_w, *k_w;      // head norms or NULL
+    float eps;
+    uint32_t n_rot, interleaved, pos0;
+    double log2_base;
+};
+hipError_t launch_kv_append(const AttnArgs &a, const RopeArgs &r, uint32_t type, uint32_t head_dim, hipStream_t s);
+
 }  // namespace kq

@@ -72,4 +72,52 @@ inline bool down_plan(bool q6, uint32_t hidden, uint32_t ffn, uint32_t n_slots, 
     return true;
 }
 
+// How an attention call's rows and keys are spread over workgroups (k_attn).
+// The rows of one key head of a sequence (query rows x the heads that share
+// the key head) make tiles of 16; with `rows` a workgroup takes four tiles,
+// else one. Keys are split where the tiles alone would leave CUs idle, into
+// parts of at least min_chunk keys; the parts' sums then meet in `slots`
+// partial results of each row. A shared prefix is either an item of its own
+// for the rows of all sequences together (shared_tiles > 0) or walked by each
+// sequence's items ahead of its own keys.
+struct AttnPlan {
+    bool rows;
+    uint32_t own_tiles, own_splits, own_items;
+    uint32_t shared_tiles, shared_splits, shared_items;
+    uint32_t slots, min_chunk;
+};
+constexpr uint32_t ATTN_MAX_SLOTS = 64;
+constexpr uint64_t ATTN_SCRATCH = 64ull << 20;   // partial results: head_dim sums, a maximum and a sum each
+
+inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint32_t n_kv, uint32_t group,
+                          uint32_t max_kv, uint32_t n_shared, uint32_t head_dim, uint32_t cus) {
+    AttnPlan p = {};
+    const uint64_t per_seq = (uint64_t)max_q * group, n_head = (uint64_t)n_kv * group;
+    const uint64_t most_slots = ATTN_SCRATCH / ((uint64_t)n_rows * n_head * (head_dim + 2) * 4);
+    p.min_chunk = 128;
+    p.rows = per_seq > 32;
+    const uint32_t tile = p.rows ? 64 : 16;
+    p.own_tiles = (uint32_t)((per_seq + tile - 1) / tile);
+    auto splits = [&](uint64_t items, uint64_t keys, uint64_t most) -> uint32_t {
+        uint64_t n = 2ull * cus / (items ? items : 1);
+        n = n < (keys + p.min_chunk - 1) / p.min_chunk ? n : (keys + p.min_chunk - 1) / p.min_chunk;
+        n = n < most ? n : most;
+        return n < 1 ? 1 : (uint32_t)n;
+    };
+    const uint64_t own = (uint64_t)n_seq * n_kv * p.own_tiles;
+    const uint64_t cap = most_slots < ATTN_MAX_SLOTS ? most_slots : ATTN_MAX_SLOTS;
+    if (n_shared && n_seq > 1 && !p.rows && cap >= 2) {
+        p.shared_tiles = (uint32_t)(((uint64_t)n_rows * group + tile - 1) / tile);
+        p.shared_splits = splits((uint64_t)n_kv * p.shared_tiles, n_shared, cap / 2);
+        p.own_splits = splits(own, max_kv, cap - p.shared_splits);
+        p.slots = p.shared_splits + p.own_splits;
+    } else {
+        p.own_splits = splits(own, (uint64_t)max_kv + n_shared, cap);
+        p.slots = p.own_splits > 1 ? p.own_splits : 0;
+    }
+    p.own_items = (uint32_t)own * p.own_splits;
+    p.shared_items = n_kv * p.shared_tiles * p.shared_splits;
+    return p;
+}
+
 }  // namespace kq

@@ -118,6 +118,10 @@ static int load(void) {
     LOAD(stager_mark, "katali_hip_stager_mark");
     LOAD(stager_upload, "katali_hip_stager_upload");
     LOAD(stager_fence, "katali_hip_stager_fence");
+    LOAD(kv_append, "katali_hip_kv_append");
+    LOAD(attn, "katali_hip_attn");
+    LOAD(attn_shared, "katali_hip_attn_shared");
+    LOAD(attn_check, "katali_hip_attn_check");
     if (g_api.abi_version() != KATALI_HIP_ABI_VERSION) {
         snprintf(g_status, sizeof g_status, "%s: ABI version %d, loader expects %d", tried, g_api.abi_version(),
                  KATALI_HIP_ABI_VERSION);
@@ -206,6 +210,18 @@ int katali_gpu_rmsnorm_matvec_f32(const float *x, const float *delta, float scal
 int katali_gpu_moe_batch(const KataliHipMoe *moe, const KataliHipMoeBatch *batch, const float *x, float *y) {
     FORWARD(g_api.moe_batch(moe, batch, x, y));
 }
+int katali_gpu_kv_append(const KataliHipAttn *a, const KataliHipRope *r, const float *q, const float *k_new,
+                         const float *v_new, float *q_out, void *k, void *v) {
+    FORWARD(g_api.kv_append(a, r, q, k_new, v_new, q_out, k, v));
+}
+int katali_gpu_attn(const KataliHipAttn *a, const float *q, const void *k, const void *v, float *out) {
+    FORWARD(g_api.attn(a, q, k, v, out));
+}
+int katali_gpu_attn_shared(const KataliHipAttn *a, const KataliHipAttnPrefix *p, const float *q, const void *k,
+                           const void *v, float *out) {
+    FORWARD(g_api.attn_shared(a, p, q, k, v, out));
+}
+int katali_gpu_attn_check(const KataliHipAttn *a, const KataliHipAttnPrefix *p) { FORWARD(g_api.attn_check(a, p)); }
 int katali_gpu_stager_create(uint64_t chunk_bytes, uint32_t n_chunks, void **stager) {
     FORWARD(g_api.stager_create(chunk_bytes, n_chunks, stager));
 }

@@ -15,6 +15,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 DEFAULT_SO = os.path.join(PKG, "libkatali_hip.so")
 
 Q4_K, Q6_K = 12, 14
+F32, F16, BF16 = 0, 1, 30   # attention caches
 BLOCK_BYTES = {Q4_K: 144, Q6_K: 210}
 
 _vp, _u64, _u32, _i32, _i64, _f32, _sz = (C.c_void_p, C.c_uint64, C.c_uint32, C.c_int32, C.c_int64,
@@ -74,6 +75,10 @@ SIGNATURES = {
     "katali_hip_phase_stamps": (C.c_int, [_vp, _sz]),
     "katali_hip_stream_floor": (C.c_int, [_i32, _vp, _sz, _vp, _sz, _vp]),
     "katali_hip_exchange_probe": (C.c_int, [_i32, C.c_uint32, _vp]),
+    "katali_hip_attn": (C.c_int, [_vp, _vp, _vp, _vp, _vp]),
+    "katali_hip_attn_shared": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "katali_hip_attn_check": (C.c_int, [_vp, _vp]),
+    "katali_hip_kv_append": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "katali_hip_stager_create": (C.c_int, [_u64, _u32, C.POINTER(_vp)]),
     "katali_hip_stager_destroy": (C.c_int, [_vp]),
     "katali_hip_stager_mark": (C.c_int, [_vp, C.POINTER(_u64)]),
@@ -105,6 +110,24 @@ class KataliHipMoeStackLayer(C.Structure):
                 ("gate_shexp", _vp), ("up_shexp", _vp), ("down_shexp", _vp), ("route", KataliHipMoeRoute),
                 ("norm_w", _vp), ("router", _vp), ("y", _vp), ("x_out", _vp), ("xn_out", _vp),
                 ("logits_out", _vp)]
+
+
+class KataliHipAttn(C.Structure):
+    _fields_ = [("struct_size", _u32), ("kv_type", _u32), ("n_head", _u32), ("n_kv_head", _u32), ("head_dim", _u32),
+                ("n_seq", _u32), ("n_rows", _u32), ("max_q", _u32), ("max_kv", _u32), ("causal", _u32),
+                ("q_start", _vp), ("kv_len", _vp), ("kv_seq_stride", _u64), ("kv_row_stride", _u64),
+                ("kv_head_stride", _u64), ("scale", _f32), ("softcap", _f32), ("slopes", _vp), ("prefix_len", _vp),
+                ("doc_start", _vp), ("doc_end", _vp)]
+
+
+class KataliHipAttnPrefix(C.Structure):
+    _fields_ = [("struct_size", _u32), ("n_prefix", _u32), ("k", _vp), ("v", _vp), ("row_stride", _u64),
+                ("head_stride", _u64)]
+
+
+class KataliHipRope(C.Structure):
+    _fields_ = [("struct_size", _u32), ("n_rot", _u32), ("interleaved", _u32), ("pos0", _u32), ("base", _f32),
+                ("eps", _f32), ("q_norm_w", _vp), ("k_norm_w", _vp)]
 
 
 # error codes of include/katali_hip.h
@@ -365,6 +388,51 @@ class KataliHip:
         b = KataliHipMoeBatch(C.sizeof(KataliHipMoeBatch), n_tokens, n_sel, mfma_min_tokens,
                               None if ids is None else ids.ptr, None if weights is None else weights.ptr)
         self.check(self.lib.katali_hip_moe_batch(C.byref(desc), C.byref(b), x.ptr, y.ptr))
+
+    # -- attention --------------------------------------------------------
+    @staticmethod
+    def attn_desc(kv_type, n_head, n_kv_head, head_dim, n_seq, kv_len, max_kv, kv_seq_stride, kv_row_stride,
+                  kv_head_stride, scale, n_rows=None, max_q=1, q_start=None, causal=True, softcap=0.0, slopes=None,
+                  prefix_len=None, doc_start=None, doc_end=None) -> KataliHipAttn:
+        """What katali_hip_attn and its neighbours read; without q_start one row per sequence."""
+        p = lambda b: None if b is None else b.ptr  # noqa: E731
+        d = KataliHipAttn(C.sizeof(KataliHipAttn), kv_type, n_head, n_kv_head, head_dim, n_seq,
+                          n_seq if n_rows is None else n_rows, max_q, max_kv, 1 if causal else 0, p(q_start),
+                          p(kv_len), kv_seq_stride, kv_row_stride, kv_head_stride, scale, softcap, p(slopes),
+                          p(prefix_len), p(doc_start), p(doc_end))
+        d._keep = (q_start, kv_len, slopes, prefix_len, doc_start, doc_end)   # as in moe_desc
+        return d
+
+    @staticmethod
+    def attn_prefix(n_prefix, k, v, row_stride, head_stride) -> KataliHipAttnPrefix:
+        d = KataliHipAttnPrefix(C.sizeof(KataliHipAttnPrefix), n_prefix, k.ptr, v.ptr, row_stride, head_stride)
+        d._keep = (k, v)
+        return d
+
+    @staticmethod
+    def rope(n_rot, base, interleaved=False, pos0=0, eps=1e-6, q_norm_w=None, k_norm_w=None) -> KataliHipRope:
+        p = lambda b: None if b is None else b.ptr  # noqa: E731
+        d = KataliHipRope(C.sizeof(KataliHipRope), n_rot, 1 if interleaved else 0, pos0, base, eps, p(q_norm_w),
+                          p(k_norm_w))
+        d._keep = (q_norm_w, k_norm_w)
+        return d
+
+    def attn(self, desc, q, k, v, out) -> None:
+        """out = attention of the packed rows q over the caches k and v."""
+        self.check(self.lib.katali_hip_attn(C.byref(desc), q.ptr, k.ptr, v.ptr, out.ptr))
+
+    def attn_shared(self, desc, prefix, q, k, v, out) -> None:
+        """The same with a prefix that all sequences share before their own keys."""
+        self.check(self.lib.katali_hip_attn_shared(C.byref(desc), C.byref(prefix), q.ptr, k.ptr, v.ptr, out.ptr))
+
+    def attn_check(self, desc, prefix=None) -> None:
+        """Raises HipError when the descriptors would be refused; needs no device."""
+        self.check(self.lib.katali_hip_attn_check(C.byref(desc), None if prefix is None else C.byref(prefix)))
+
+    def kv_append(self, desc, rope, q, k_new, v_new, q_out, k, v) -> None:
+        """Norm and turn the rows' q and k, store k and v in the caches."""
+        self.check(self.lib.katali_hip_kv_append(C.byref(desc), C.byref(rope), q.ptr, k_new.ptr, v_new.ptr, q_out.ptr,
+                                                 k.ptr, v.ptr))
 
     def argmax(self, logits: DeviceBuffer, n: int, out: DeviceBuffer) -> None:
         self.check(self.lib.katali_hip_argmax(logits.ptr, n, out.ptr))
