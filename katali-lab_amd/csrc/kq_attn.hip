@@ -20,9 +20,8 @@
 // whose B operand is P^T in the very registers that S^T came in: the keys of
 // an operand may stand in any order if both operands have the same. V^T's
 // operand wants four keys of one column in a lane; a lane loads 4 rows of V,
-// D/16 columns each, and exchanges halves between them (v_perm), no LDS. The
-// four waves of a workgroup share 16 rows and take every fourth tile (few
-// rows: the keys are what there is to spread), or take 64 rows.
+// D/16 columns each, and exchanges halves between them (v_perm), no LDS.
+// k_attn_tile: the same for many rows, the keys staged through LDS.
 #include <type_traits>
 
 #include "kq_attn.h"
@@ -33,6 +32,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float NEG_INF = -__builtin_inff();
@@ -83,7 +83,7 @@ __device__ __forceinline__ void split(float x, float y, uint32_t (&w)[TERMS<TY>]
     if constexpr (TY == ATTN_F16) {
         const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
         w[0] = bits<uint32_t>(h);
-        w[1] = bits<uint32_t>(__builtin_amdgcn_cvt_pkrtz(x - (float)h[0], y - (float)h[1]));
+        w[1] = bits<uint32_t>(__builtin_amdgcn_cvt_pkrtz(fmaf((float)h[0], -1.0f, x), fmaf((float)h[1], -1.0f, y)));
     } else {
 #pragma unroll
         for (int n = 0; n < 3; n++) {
@@ -115,6 +115,7 @@ struct Score {
     float mul;     // product -> score (with a cap: -> score / cap)
     float cap;     // cap log2(e), 0 for none
     float slope;   // slope log2(e)
+    bool bare;     // neither cap nor bias, and a positive factor (the same for all rows)
 };
 __device__ __forceinline__ float score(const Score &c, float s, int32_t pos, int32_t j) {
     float y = s * c.mul;
@@ -218,6 +219,16 @@ struct Frag {
                            c * (G::DPL * G::EB));
         }
     }
+    __device__ __forceinline__ uint4 key(int t, int i) const { return k[t][i]; }
+    // V^T's operand for columns DPL (l % 16) + t: halves of 4 + 4 rows exchanged
+    __device__ __forceinline__ uint4 value(int t) const {
+        const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = __builtin_amdgcn_perm(v[2 * i + 1][t / 2], v[2 * i][t / 2], sel);
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ __forceinline__ float value(int r, int t) const { return __uint_as_float(v[r][t]); }
     __device__ __forceinline__ void ldv(int r, const char *p) {
         if constexpr (G::VW >= 4) {
 #pragma unroll
@@ -286,6 +297,7 @@ struct Wave16 {
         sc.cap = a.softcap * LOG2E;
         sc.mul = a.softcap != 0.0f ? mul / a.softcap : mul * LOG2E;
         sc.slope = a.slopes && r.valid ? a.slopes[r.head] * LOG2E : 0.0f;
+        sc.bare = a.softcap == 0.0f && !a.slopes && !__any(!(sc.mul > 0.0f));
         m = NEG_INF;
         l = 0.0f;
 #pragma unroll
@@ -294,8 +306,8 @@ struct Wave16 {
 
     // keys j0 .. j0 + KT of one tile, those from `end` on not of its segment;
     // whole: every row sees all of them
-    __device__ __forceinline__ void step(const Frag<TY, D> &f, const Row &row, int32_t j0, int32_t end, bool whole,
-                                         int lane) {
+    template <class Src>
+    __device__ __forceinline__ void step(const Src &f, const Row &row, int32_t j0, int32_t end, bool whole, int lane) {
         const int32_t g4 = 4 * (lane >> 4);
         float y[G::VR];
 #pragma unroll
@@ -303,17 +315,27 @@ struct Wave16 {
             f32x4 s = {0, 0, 0, 0};
 #pragma unroll
             for (int c = 0; c < G::KC; c++) {
+                const uint4 k = f.key(t, c);
                 if constexpr (TY == ATTN_F32) {
-                    const f32x4 kv = bits<f32x4>(f.k[t][c]), qv = bits<f32x4>(q[0][c]);
+                    const f32x4 kv = bits<f32x4>(k), qv = bits<f32x4>(q[0][c]);
 #pragma unroll
                     for (int i = 0; i < 4; i++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[i], qv[i], s, 0, 0, 0);
                 } else {
 #pragma unroll
-                    for (int n = 0; n < NT; n++) s = mfma32<TY>(f.k[t][c], q[n][c], s);
+                    for (int n = 0; n < NT; n++) s = mfma32<TY>(k, q[n][c], s);
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[4 * t + r] = score(sc, s[r], row.pos, j0 + 16 * t + g4 + r);
+            for (int r = 0; r < 4; r++) y[4 * t + r] = s[r];
+        }
+        // with neither cap nor bias the product's factor goes into the exponent's
+        // multiply-add, and y stays the bare product
+        float mul = 1.0f;
+        if (sc.bare) {
+            mul = sc.mul;
+        } else {
+#pragma unroll
+            for (int r = 0; r < G::VR; r++) y[r] = score(sc, y[r], row.pos, j0 + 16 * (r >> 2) + g4 + (r & 3));
         }
         if (!whole) {
             const int32_t hi = min(row.hi, end);
@@ -326,7 +348,7 @@ struct Wave16 {
         float top = y[0];
 #pragma unroll
         for (int r = 1; r < G::VR; r++) top = fmaxf(top, y[r]);
-        top = rows_max(top);
+        top = rows_max(top) * mul;
         // the maximum that scales the sums moves only when it falls behind by
         // 2^8: most tiles then leave the accumulators alone
         if (__any(top > m + 8.0f)) {
@@ -342,7 +364,7 @@ struct Wave16 {
         float p[G::VR];
 #pragma unroll
         for (int r = 0; r < G::VR; r++) {
-            p[r] = exp2_hw(y[r] - base);
+            p[r] = exp2_hw(fmaf(y[r], mul, -base));
             l += p[r];
         }
         if constexpr (TY == ATTN_F32) {
@@ -350,19 +372,14 @@ struct Wave16 {
             for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int t = 0; t < G::DPL; t++)
-                    o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.v[r][t]), p[r], o[t], 0, 0, 0);
+                    o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.value(r, t), p[r], o[t], 0, 0, 0);
         } else {
             uint32_t pt[4][NT];
 #pragma unroll
             for (int i = 0; i < 4; i++) split<TY>(p[2 * i], p[2 * i + 1], pt[i]);
 #pragma unroll
             for (int t = 0; t < G::DPL; t++) {
-                const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    w[i] = __builtin_amdgcn_perm(f.v[2 * i + 1][t / 2], f.v[2 * i][t / 2], sel);
-                const uint4 vt = make_uint4(w[0], w[1], w[2], w[3]);
+                const uint4 vt = f.value(t);
 #pragma unroll
                 for (int n = 0; n < NT; n++)
                     o[t] = mfma32<TY>(vt, make_uint4(pt[0][n], pt[1][n], pt[2][n], pt[3][n]), o[t]);
@@ -424,6 +441,7 @@ __device__ __forceinline__ void row_again(const AttnArgs &a, uint32_t kvh, uint3
     sc.cap = a.softcap * LOG2E;
     sc.mul = a.softcap != 0.0f ? a.scale / a.softcap : a.scale * LOG2E;
     sc.slope = a.slopes ? a.slopes[r.head] * LOG2E : 0.0f;
+    sc.bare = false;
     m = NEG_INF;
     l = 0.0f;
 #pragma unroll
@@ -482,68 +500,115 @@ __device__ __forceinline__ uint64_t slot_of(const AttnArgs &a, uint64_t rh, cons
     return rh * a.slots + (it.pooled ? a.own_splits : 0) + it.split;
 }
 
-// RS: the four waves take four row tiles and all keys of the item; else one
-// row tile and every fourth key tile.
-template <int TY, int D, bool RS>
-__global__ void __launch_bounds__(256, D <= (TY == ATTN_BF16 ? 64 : 128) ? 2 : 1) k_attn(const AttnArgs a) {
-    using G = Tile<TY, D>;
-    constexpr int W = 4;
-    __shared__ float lds_o[RS ? 1 : W][RS ? 1 : 16][RS ? 1 : D + 4];
-    __shared__ float lds_m[W][16], lds_l[W][16];
-    __shared__ float lds_row[W][D];
-    __shared__ uint64_t lds_at[16];   // packed row x head of each tile row, ~0 for none
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Item it = make_item(a, blockIdx.x);
-
-    SeqRows sr;
-    int32_t n_row;
+// The rows an item's packed rows are counted from, and how many there are.
+__device__ __forceinline__ int32_t item_rows(const AttnArgs &a, const Item &it, SeqRows &sr) {
     if (it.pooled) {
         sr.first = a.q_start ? min(max(a.q_start[0], 0), (int32_t)a.n_rows) : 0;
         sr.last = a.q_start ? min(max(a.q_start[a.n_seq], sr.first), (int32_t)a.n_rows) : (int32_t)a.n_rows;
         sr.len = 0;
-        n_row = sr.last - sr.first;
-    } else {
-        sr = seq_rows(a, it.seq);
-        n_row = min(sr.last - sr.first, (int32_t)a.max_q);
+        return sr.last - sr.first;
     }
-    const uint32_t first = (it.tile * (RS ? W : 1) + (RS ? wave : 0)) * 16;
-    const Row row = make_row(a, it.kvh, first + (lane & 15), it.pooled, it.seq, sr, n_row);
+    sr = seq_rows(a, it.seq);
+    return min(sr.last - sr.first, (int32_t)a.max_q);
+}
 
-    // the keys any row of the tile sees, of those this item is for, and this split's share of them
+// Of a wave's 16 rows: the keys some row sees among those the item is for,
+// [lo, hi), and the keys that every row sees, [all_lo, all_hi).
+struct Span {
+    int32_t lo, hi, all_lo, all_hi;
+};
+__device__ __forceinline__ Span wave_span(const AttnArgs &a, const Item &it, const SeqRows &sr, const Row &row) {
     int32_t kb = 0, ke = (int32_t)a.n_shared + sr.len;
     if (it.pooled) ke = (int32_t)a.n_shared;
     else if (a.shared_splits) kb = (int32_t)a.n_shared;
     const int32_t rl = max(row.lo, kb), rh = min(row.hi, ke);
     const bool some = rl < rh;
-    const int32_t tl = __builtin_amdgcn_readfirstlane(row16_min(some ? rl : INT32_MAX));
-    const int32_t th = __builtin_amdgcn_readfirstlane(-row16_min(some ? -rh : 0));
-    // keys that every row sees: tiles inside need no mask
-    const int32_t al = __builtin_amdgcn_readfirstlane(-row16_min(row.valid ? -row.lo : 0));
-    const int32_t ah = __builtin_amdgcn_readfirstlane(row16_min(row.valid ? row.hi : INT32_MAX));
-    int32_t c0 = 0, c1 = 0;
-    if (th > tl) {
-        const uint32_t n = (uint32_t)(th - tl), splits = it.pooled ? a.shared_splits : a.own_splits;
-        const uint32_t used = min(max((n + a.min_chunk - 1) / a.min_chunk, 1u), splits);
-        const uint32_t chunk = ((n + used - 1) / used + G::KT - 1) / G::KT * G::KT;
-        const uint64_t b = (uint64_t)it.split * chunk;
-        if (b < n) {
-            c0 = tl + (int32_t)b;
-            c1 = tl + (int32_t)min((uint64_t)n, b + chunk);
-        }
+    Span s;
+    s.lo = __builtin_amdgcn_readfirstlane(row16_min(some ? rl : INT32_MAX));
+    s.hi = __builtin_amdgcn_readfirstlane(-row16_min(some ? -rh : 0));
+    s.all_lo = __builtin_amdgcn_readfirstlane(-row16_min(row.valid ? -row.lo : 0));
+    s.all_hi = __builtin_amdgcn_readfirstlane(row16_min(row.valid ? row.hi : INT32_MAX));
+    return s;
+}
+
+// A split's share [c0, c1) of the keys [lo, hi), in whole tiles of `tile` keys.
+__device__ __forceinline__ void split_share(const AttnArgs &a, const Item &it, int32_t lo, int32_t hi, uint32_t tile,
+                                            int32_t &c0, int32_t &c1) {
+    c0 = c1 = 0;
+    if (hi <= lo) return;
+    const uint32_t n = (uint32_t)(hi - lo), splits = it.pooled ? a.shared_splits : a.own_splits;
+    const uint32_t used = min(max((n + a.min_chunk - 1) / a.min_chunk, 1u), splits);
+    const uint32_t chunk = ((n + used - 1) / used + tile - 1) / tile * tile;
+    const uint64_t b = (uint64_t)it.split * chunk;
+    if (b < n) {
+        c0 = lo + (int32_t)b;
+        c1 = lo + (int32_t)min((uint64_t)n, b + chunk);
     }
+}
+
+// Rows of the wave that met an infinity or NaN, key by key; buf: D floats of LDS of the wave's own.
+template <int TY, int D, int W>
+__device__ __forceinline__ void odd_rows(const AttnArgs &a, const Item &it, const Row &row, int32_t c0, int32_t c1,
+                                         int wave, int lane, Wave16<TY, D> &st, float *buf) {
+    using G = Tile<TY, D>;
+    uint64_t odd = __ballot(row.valid && st.odd());
+    odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xFFFF;
+    while (odd) {
+        const int i = __builtin_ctzll(odd);
+        odd &= odd - 1;
+        Row r;
+        r.row = __builtin_amdgcn_readlane(row.row, i);
+        r.pos = __builtin_amdgcn_readlane(row.pos, i);
+        r.lo = __builtin_amdgcn_readlane(row.lo, i);
+        r.hi = __builtin_amdgcn_readlane(row.hi, i);
+        r.head = (uint32_t)__builtin_amdgcn_readlane((int)row.head, i);
+        r.valid = true;
+        float acc[D / 64], m, l;
+        row_again<TY, D, W>(a, it.kvh, it.seq, r, c0, c1, wave, lane, acc, m, l);
+#pragma unroll
+        for (int e = 0; e < D / 64; e++) buf[lane + 64 * e] = acc[e];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if ((lane & 15) == i) {
+            st.m = m;
+            st.l = l;
+#pragma unroll
+            for (int t = 0; t < G::DPL; t++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) st.o[t][q] = buf[G::DPL * (4 * (lane >> 4) + q) + t];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
+// Few rows: the four waves of a workgroup share 16 rows and take every fourth tile of the keys.
+template <int TY, int D>
+__global__ void __launch_bounds__(256, D <= (TY == ATTN_BF16 ? 64 : 128) ? 2 : 1) k_attn(const AttnArgs a) {
+    using G = Tile<TY, D>;
+    constexpr int W = 4;
+    __shared__ float lds_o[W][16][D + 4];
+    __shared__ float lds_m[W][16], lds_l[W][16];
+    __shared__ float lds_row[W][D];
+    __shared__ uint64_t lds_at[16];   // packed row x head of each tile row, ~0 for none
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Item it = make_item(a, blockIdx.x);
+    SeqRows sr;
+    const int32_t n_row = item_rows(a, it, sr);
+    const Row row = make_row(a, it.kvh, it.tile * 16 + (lane & 15), it.pooled, it.seq, sr, n_row);
+    const Span sp = wave_span(a, it, sr, row);
+    int32_t c0, c1;
+    split_share(a, it, sp.lo, sp.hi, G::KT, c0, c1);
 
     Wave16<TY, D> st;
     st.init(a, row, lane);
     for (int sg = 0; sg < 2; sg++) {
         const Segment g = segment(a, G::EB, it.kvh, it.seq, sg == 0, c0, c1);
-        const int32_t step = (RS ? 1 : W) * G::KT;
-        int32_t j = g.c0 + (RS ? 0 : wave * G::KT);
+        int32_t j = g.c0 + wave * G::KT;
         if (j >= g.c1) continue;
         Frag<TY, D> f;
         f.load(g.k, g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
         while (true) {
-            const int32_t jn = j + step;
-            const bool whole = j >= al && j + G::KT <= min(ah, g.c1);
+            const int32_t jn = j + W * G::KT;
+            const bool whole = j >= sp.all_lo && j + G::KT <= min(sp.all_hi, g.c1);
             if constexpr (D <= 128) {
                 Frag<TY, D> fn;
                 if (jn < g.c1) fn.load(g.k, g.v, g.row_bytes, jn - g.origin, g.c1 - g.origin, lane);
@@ -558,105 +623,232 @@ __global__ void __launch_bounds__(256, D <= (TY == ATTN_BF16 ? 64 : 128) ? 2 : 1
         }
     }
     st.l = rows_sum(st.l);
+    odd_rows<TY, D, W>(a, it, row, c0, c1, wave, lane, st, lds_row[wave]);
 
-    // rows that met an infinity or NaN, key by key
-    uint64_t odd = __ballot(st.odd());
-    odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xFFFF;
-    while (odd) {
-        const int i = __builtin_ctzll(odd);
-        odd &= odd - 1;
-        Row r;
-        r.row = __builtin_amdgcn_readlane(row.row, i);
-        r.pos = __builtin_amdgcn_readlane(row.pos, i);
-        r.lo = __builtin_amdgcn_readlane(row.lo, i);
-        r.hi = __builtin_amdgcn_readlane(row.hi, i);
-        r.head = (uint32_t)__builtin_amdgcn_readlane((int)row.head, i);
-        r.valid = true;
-        float acc[D / 64], m, l;
-        row_again<TY, D, RS ? 1 : W>(a, it.kvh, it.seq, r, c0, c1, RS ? 0 : wave, lane, acc, m, l);
-#pragma unroll
-        for (int e = 0; e < D / 64; e++) lds_row[wave][lane + 64 * e] = acc[e];
-        __builtin_amdgcn_wave_barrier();
-        if ((lane & 15) == i) {
-            st.m = m;
-            st.l = l;
-#pragma unroll
-            for (int t = 0; t < G::DPL; t++)
-#pragma unroll
-                for (int q = 0; q < 4; q++) st.o[t][q] = lds_row[wave][G::DPL * (4 * (lane >> 4) + q) + t];
-        }
-        __builtin_amdgcn_wave_barrier();
+    // the four waves' sums of the same rows, joined in LDS
+    if (lane < 16) {
+        lds_m[wave][lane] = st.m;
+        lds_l[wave][lane] = st.l;
+        if (wave == 0) lds_at[lane] = row.valid ? row_head(a, row) : ~0ull;
     }
-
-    if constexpr (RS) {
-        if (!row.valid) return;
-        float *dst;
-        float f0 = 1.0f;
-        if (a.slots) {
-            const uint64_t at = slot_of(a, row_head(a, row), it);
-            if (lane < 16) a.ml[at] = make_float2(st.m, st.l);
-            dst = a.acc + at * D;
-            if (st.l == 0.0f) return;
-        } else {
-            f0 = st.l == 0.0f ? 0.0f : 1.0f / st.l;
-            dst = a.out + row_head(a, row) * D;
-        }
 #pragma unroll
-        for (int q = 0; q < 4; q++)
+    for (int q = 0; q < 4; q++)
 #pragma unroll
-            for (int t = 0; t < G::DPL; t += 4)
-                *(float4 *)(dst + G::DPL * (4 * (lane >> 4) + q) + t) =
-                    make_float4(st.o[t][q] * f0, st.o[t + 1][q] * f0, st.o[t + 2][q] * f0, st.o[t + 3][q] * f0);
+        for (int t = 0; t < G::DPL; t += 4)
+            *(float4 *)&lds_o[wave][lane & 15][G::DPL * (4 * (lane >> 4) + q) + t] =
+                make_float4(st.o[t][q], st.o[t + 1][q], st.o[t + 2][q], st.o[t + 3][q]);
+    __syncthreads();
+    // thread: row tid / 16, columns D/16 (tid % 16) ...
+    const int i = threadIdx.x >> 4;
+    const uint64_t rh = lds_at[i];
+    if (rh == ~0ull) return;
+    float m = NEG_INF, l = 0.0f, w[W];
+#pragma unroll
+    for (int k = 0; k < W; k++) m = fmaxf(m, lds_m[k][i]);
+#pragma unroll
+    for (int k = 0; k < W; k++) {
+        w[k] = lds_l[k][i] == 0.0f ? 0.0f : exp2_hw(lds_m[k][i] - m);
+        l += lds_l[k][i] * w[k];
+    }
+    float *dst;
+    float f0 = 1.0f;
+    if (a.slots) {
+        const uint64_t at = slot_of(a, rh, it);
+        if ((threadIdx.x & 15) == 0) a.ml[at] = make_float2(m, l);
+        if (l == 0.0f) return;
+        dst = a.acc + at * D;
     } else {
-        // the four waves' sums of the same rows, joined in LDS
-        if (lane < 16) {
-            lds_m[wave][lane] = st.m;
-            lds_l[wave][lane] = st.l;
-            if (wave == 0) lds_at[lane] = row.valid ? row_head(a, row) : ~0ull;
-        }
+        f0 = l == 0.0f ? 0.0f : 1.0f / l;
+        dst = a.out + rh * D;
+    }
 #pragma unroll
-        for (int q = 0; q < 4; q++)
-#pragma unroll
-            for (int t = 0; t < G::DPL; t += 4)
-                *(float4 *)&lds_o[wave][lane & 15][G::DPL * (4 * (lane >> 4) + q) + t] =
-                    make_float4(st.o[t][q], st.o[t + 1][q], st.o[t + 2][q], st.o[t + 3][q]);
-        __syncthreads();
-        // thread: row tid / 16, columns D/16 (tid % 16) ...
-        const int i = threadIdx.x >> 4;
-        const uint64_t rh = lds_at[i];
-        if (rh == ~0ull) return;
-        float m = NEG_INF, l = 0.0f, w[W];
-#pragma unroll
-        for (int k = 0; k < W; k++) m = fmaxf(m, lds_m[k][i]);
+    for (int t = 0; t < G::DPL; t += 4) {
+        const int col = (threadIdx.x & 15) * G::DPL + t;
+        float x[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < W; k++) {
-            w[k] = lds_l[k][i] == 0.0f ? 0.0f : exp2_hw(lds_m[k][i] - m);
-            l += lds_l[k][i] * w[k];
+            if (w[k] == 0.0f) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = fmaf(lds_o[k][i][col + e], w[k], x[e]);
         }
-        float *dst;
-        float f0 = 1.0f;
-        if (a.slots) {
-            const uint64_t at = slot_of(a, rh, it);
-            if ((threadIdx.x & 15) == 0) a.ml[at] = make_float2(m, l);
-            if (l == 0.0f) return;
-            dst = a.acc + at * D;
-        } else {
-            f0 = l == 0.0f ? 0.0f : 1.0f / l;
-            dst = a.out + rh * D;
-        }
+        *(float4 *)(dst + col) = make_float4(x[0] * f0, x[1] * f0, x[2] * f0, x[3] * f0);
+    }
+}
+
+// Keys and values of NK keys in LDS, for all waves of a workgroup. K row by
+// row, 16 bytes of padding each: the 16 rows that a wave's lanes read 16 bytes
+// of lie in different banks. 16-bit V in the order of the operand that V^T's
+// product takes (column tile, lane, 8 keys): a thread loads 4 rows of 4
+// columns and exchanges halves once, where every wave would do it again. fp32
+// V row by row.
+template <int TY, int D, int NTHREADS>
+struct Stage {
+    using G = Tile<TY, D>;
+    static constexpr int NK = TY == ATTN_F32 || (TY == ATTN_BF16 && D == 256) ? 32 : 64;   // 32: registers
+    static constexpr int KROW = D * G::EB + 16, VBYTES = TY == ATTN_F32 ? NK * KROW : NK * D * 2;
+    static constexpr int BYTES = NK * KROW + VBYTES;
+    static constexpr int PER_ROW = D * G::EB / 16;                            // 16-byte pieces of a row
+    static constexpr int KN = NK * PER_ROW / NTHREADS;                        // pieces of K per thread
+    static constexpr int UNITS = NK / 4 * (D / 4);                            // 4 x 4 blocks of V
+    static constexpr int VN = (UNITS + NTHREADS - 1) / NTHREADS;              // blocks per thread
+    static_assert(NK * PER_ROW % NTHREADS == 0, "whole pieces per thread");
+
+    u32x4 k[KN];
+    uint2 v[TY == ATTN_F32 ? 2 * KN : VN * 4];
+
+    // rows j0 .. j0 + NK from memory; rows from `end` on repeat the last one before it
+    __device__ __forceinline__ void fetch(const char *kb, const char *vb, uint32_t row_bytes, int32_t j0, int32_t end) {
+        const uint64_t at = (uint64_t)(uint32_t)j0 * row_bytes;
+        const char *kp = kb + at, *vp = vb + at;
+        const uint32_t last = (uint32_t)min(end - j0, NK) - 1;
 #pragma unroll
-        for (int t = 0; t < G::DPL; t += 4) {
-            const int col = (threadIdx.x & 15) * G::DPL + t;
-            float x[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int k = 0; k < W; k++) {
-                if (w[k] == 0.0f) continue;
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[e] = fmaf(lds_o[k][i][col + e], w[k], x[e]);
+        for (int n = 0; n < KN; n++) {
+            const uint32_t id = threadIdx.x + NTHREADS * n;
+            const uint32_t off = min(id / PER_ROW, last) * row_bytes + id % PER_ROW * 16;
+            k[n] = *(const u32x4 *)(kp + off);
+            if constexpr (TY == ATTN_F32) {
+                const uint4 x = *(const uint4 *)(vp + off);
+                v[2 * n] = make_uint2(x.x, x.y), v[2 * n + 1] = make_uint2(x.z, x.w);
             }
-            *(float4 *)(dst + col) = make_float4(x[0] * f0, x[1] * f0, x[2] * f0, x[3] * f0);
+        }
+        if constexpr (TY != ATTN_F32) {
+#pragma unroll
+            for (int n = 0; n < VN; n++) {
+                const uint32_t id = threadIdx.x + NTHREADS * n;
+                if (UNITS % NTHREADS == 0 || id < UNITS) {
+                    const uint32_t rows = id / (D / 4) * 4, col = id % (D / 4) * 8;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) v[4 * n + r] = *(const uint2 *)(vp + min(rows + r, last) * row_bytes + col);
+                }
+            }
         }
     }
+    __device__ __forceinline__ void store(char *lds) const {
+#pragma unroll
+        for (int n = 0; n < KN; n++) {
+            const uint32_t id = threadIdx.x + NTHREADS * n;
+            *(u32x4 *)(lds + id / PER_ROW * KROW + id % PER_ROW * 16) = k[n];
+            if constexpr (TY == ATTN_F32)
+                *(uint4 *)(lds + NK * KROW + id / PER_ROW * KROW + id % PER_ROW * 16) =
+                    make_uint4(v[2 * n].x, v[2 * n].y, v[2 * n + 1].x, v[2 * n + 1].y);
+        }
+        if constexpr (TY != ATTN_F32) {
+#pragma unroll
+            for (int n = 0; n < VN; n++) {
+                const uint32_t id = threadIdx.x + NTHREADS * n;
+                if (UNITS % NTHREADS == 0 || id < UNITS) {
+                    // rows 4 q .. of subtile q / 8: half (q / 4) % 2 of the operand's keys, lane row q % 4
+                    const uint32_t q = id / (D / 4), col = id % (D / 4) * 4;
+                    const uint32_t sub = q / 8, half = q / 4 % 2, lane0 = q % 4 * 16 + col / G::DPL, t0 = col % G::DPL;
+                    char *p = lds + NK * KROW + sub * (32 * D * 2) + (t0 * 64 + lane0) * 16 + half * 8;
+                    const uint2 *x = v + 4 * n;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+                        const uint32_t r0 = e < 2 ? x[0].x : x[0].y, r1 = e < 2 ? x[1].x : x[1].y;
+                        const uint32_t r2 = e < 2 ? x[2].x : x[2].y, r3 = e < 2 ? x[3].x : x[3].y;
+                        *(uint2 *)(p + e * 1024) =
+                            make_uint2(__builtin_amdgcn_perm(r1, r0, sel), __builtin_amdgcn_perm(r3, r2, sel));
+                    }
+                }
+            }
+        }
+    }
+    // the operands of one of its tiles, as Frag gives them
+    struct View {
+        const char *kp, *vp;
+        __device__ __forceinline__ uint4 key(int t, int i) const { return *(const uint4 *)(kp + t * 16 * KROW + i * 64); }
+        __device__ __forceinline__ uint4 value(int t) const { return *(const uint4 *)(vp + t * 1024); }
+        __device__ __forceinline__ float value(int r, int t) const { return *(const float *)(vp + r * KROW + t * 4); }
+    };
+    static __device__ __forceinline__ View view(const char *lds, int sub, int lane) {
+        View w;
+        const int c = lane & 15, g = lane >> 4;
+        w.kp = lds + (sub * G::KT + c) * KROW + g * 16;
+        if constexpr (TY == ATTN_F32) w.vp = lds + NK * KROW + (sub * G::KT + 4 * g) * KROW + c * (G::DPL * 4);
+        else w.vp = lds + NK * KROW + sub * (32 * D * 2) + lane * 16;
+        return w;
+    }
+};
+
+// Many rows: eight waves of 16 rows each walk the same keys, staged through
+// LDS for all of them (two buffers: the next keys are on their way from memory
+// while these are worked on, one barrier per stage).
+template <int TY, int D>
+__global__ void __launch_bounds__(512, 2) k_attn_tile(const AttnArgs a) {
+    using G = Tile<TY, D>;
+    constexpr int W = 8;
+    using S = Stage<TY, D, 64 * W>;
+    __shared__ __align__(16) char lds[2][S::BYTES];
+    __shared__ int32_t span[2][W];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Item it = make_item(a, blockIdx.x);
+    SeqRows sr;
+    const int32_t n_row = item_rows(a, it, sr);
+    const Row row = make_row(a, it.kvh, (it.tile * W + wave) * 16 + (lane & 15), it.pooled, it.seq, sr, n_row);
+    const Span sp = wave_span(a, it, sr, row);
+    if (lane == 0) {
+        span[0][wave] = sp.lo;
+        span[1][wave] = sp.hi;
+    }
+    __syncthreads();
+    int32_t lo = INT32_MAX, hi = 0, c0, c1;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        lo = min(lo, span[0][w]);
+        hi = max(hi, span[1][w]);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    split_share(a, it, lo, hi, S::NK, c0, c1);
+
+    Wave16<TY, D> st;
+    st.init(a, row, lane);
+    S stage;
+    for (int sg = 0; sg < 2; sg++) {
+        const Segment g = segment(a, G::EB, it.kvh, it.seq, sg == 0, c0, c1);
+        if (g.c0 >= g.c1) continue;
+        stage.fetch(g.k, g.v, g.row_bytes, g.c0 - g.origin, g.c1 - g.origin);
+        int at = 0;
+        __syncthreads();   // the last segment's readers are done
+        stage.store(lds[0]);
+        __syncthreads();
+        for (int32_t j = g.c0; j < g.c1; j += S::NK) {
+            const bool more = j + S::NK < g.c1;
+            if (more) stage.fetch(g.k, g.v, g.row_bytes, j + S::NK - g.origin, g.c1 - g.origin);
+#pragma unroll 1
+            for (int sub = 0; sub < S::NK / G::KT; sub++) {
+                const int32_t js = j + sub * G::KT;
+                if (js >= min(sp.hi, g.c1) || js + G::KT <= sp.lo) continue;
+                const bool whole = js >= sp.all_lo && js + G::KT <= min(sp.all_hi, g.c1);
+                st.step(S::view(lds[at], sub, lane), row, js, g.c1, whole, lane);
+            }
+            if (more) stage.store(lds[at ^ 1]);
+            __syncthreads();
+            at ^= 1;
+        }
+    }
+    st.l = rows_sum(st.l);
+    odd_rows<TY, D, 1>(a, it, row, c0, c1, 0, lane, st, (float *)lds[0] + wave * D);
+
+    if (!row.valid) return;
+    float *dst;
+    float f0 = 1.0f;
+    if (a.slots) {
+        const uint64_t at = slot_of(a, row_head(a, row), it);
+        if (lane < 16) a.ml[at] = make_float2(st.m, st.l);
+        dst = a.acc + at * D;
+        if (st.l == 0.0f) return;
+    } else {
+        f0 = st.l == 0.0f ? 0.0f : 1.0f / st.l;
+        dst = a.out + row_head(a, row) * D;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+        for (int t = 0; t < G::DPL; t += 4)
+            *(float4 *)(dst + G::DPL * (4 * (lane >> 4) + q) + t) =
+                make_float4(st.o[t][q] * f0, st.o[t + 1][q] * f0, st.o[t + 2][q] * f0, st.o[t + 3][q] * f0);
 }
 
 // The partial sums of a row, joined: one wave per (row, head).
@@ -693,8 +885,8 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
 
 template <int TY, int D>
 static hipError_t attn_run(const AttnArgs &a, bool rows, uint32_t items, hipStream_t s) {
-    if (rows) hipLaunchKernelGGL((k_attn<TY, D, true>), dim3(items), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_attn<TY, D, false>), dim3(items), dim3(256), 0, s, a);
+    if (rows) hipLaunchKernelGGL((k_attn_tile<TY, D>), dim3(items), dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((k_attn<TY, D>), dim3(items), dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !a.slots) return e;
     hipLaunchKernelGGL((k_attn_join<D>), dim3(a.n_seq * a.max_q * ((a.n_head + 3) / 4)), dim3(256), 0, s, a);

@@ -74,7 +74,7 @@ inline bool down_plan(bool q6, uint32_t hidden, uint32_t ffn, uint32_t n_slots, 
 
 // How an attention call's rows and keys are spread over workgroups (k_attn).
 // The rows of one key head of a sequence (query rows x the heads that share
-// the key head) make tiles of 16; with `rows` a workgroup takes four tiles,
+// the key head) make tiles of 16; with `rows` a workgroup takes eight tiles,
 // else one. Keys are split where the tiles alone would leave CUs idle, into
 // parts of at least min_chunk keys; the parts' sums then meet in `slots`
 // partial results of each row. A shared prefix is either an item of its own
@@ -96,7 +96,7 @@ inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint3
     const uint64_t most_slots = ATTN_SCRATCH / ((uint64_t)n_rows * n_head * (head_dim + 2) * 4);
     p.min_chunk = 128;
     p.rows = per_seq > 32;
-    const uint32_t tile = p.rows ? 64 : 16;
+    const uint32_t tile = p.rows ? 128 : 16;
     p.own_tiles = (uint32_t)((per_seq + tile - 1) / tile);
     auto splits = [&](uint64_t items, uint64_t keys, uint64_t most) -> uint32_t {
         uint64_t n = 2ull * cus / (items ? items : 1);
