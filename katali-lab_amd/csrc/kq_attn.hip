@@ -110,18 +110,32 @@ __device__ __forceinline__ float ld_kv(const void *p, uint64_t i) {
     else return __uint_as_float((uint32_t)((const uint16_t *)p)[i] << 16);
 }
 
-// A row's score of one key in log2 units, from the accumulated product s.
+// How the accumulated product becomes a row's score of a key, in log2 units.
+// What a call has of cap and bias is the same for all rows: scalar branches.
 struct Score {
-    float mul;     // product -> score (with a cap: -> score / cap)
-    float cap;     // cap log2(e), 0 for none
-    float slope;   // slope log2(e)
-    bool bare;     // neither cap nor bias, and a positive factor (the same for all rows)
+    float mul;      // product -> score (with a cap: -> score / cap)
+    float cap;      // cap log2(e)
+    float slope;    // -slope log2(e)
+    bool capped, sloped;
+    bool bare;      // neither, and a positive factor for every row of the wave
 };
-__device__ __forceinline__ float score(const Score &c, float s, int32_t pos, int32_t j) {
-    float y = s * c.mul;
-    if (c.cap != 0.0f) y = c.cap * tanh_fast(y);
-    if (c.slope != 0.0f) y = fmaf(-c.slope, fabsf((float)(pos - j)), y);
-    return y;
+struct Row;
+__device__ __forceinline__ Score make_score(const AttnArgs &a, const Row &r, float mul);
+// scores of the keys j0 + off(r), pos0 = position - j0
+template <int N, class Off>
+__device__ __forceinline__ void scores(const Score &c, float (&y)[N], int32_t pos0, Off off) {
+    if (c.capped) {
+#pragma unroll
+        for (int r = 0; r < N; r++) y[r] = c.cap * tanh_fast(y[r] * c.mul);
+    } else {
+#pragma unroll
+        for (int r = 0; r < N; r++) y[r] *= c.mul;
+    }
+    if (c.sloped) {
+        const float p = (float)pos0;
+#pragma unroll
+        for (int r = 0; r < N; r++) y[r] = fmaf(fabsf(p - (float)off(r)), c.slope, y[r]);
+    }
 }
 
 // What a wave's lane knows about the query row it holds (lanes 16 apart hold
@@ -161,6 +175,17 @@ __device__ __forceinline__ Row make_row(const AttnArgs &a, uint32_t kvh, uint32_
     return r;
 }
 
+__device__ __forceinline__ Score make_score(const AttnArgs &a, const Row &r, float mul) {
+    Score c;
+    c.capped = (__float_as_uint(a.softcap) << 1) != 0;
+    c.sloped = a.slopes != nullptr;
+    c.cap = a.softcap * LOG2E;
+    c.mul = c.capped ? mul / a.softcap : mul * LOG2E;
+    c.slope = c.sloped && r.valid ? a.slopes[r.head] * -LOG2E : 0.0f;
+    c.bare = !c.capped && !c.sloped && !__any(!(c.mul > 0.0f));
+    return c;
+}
+
 // min / max over the wave of an integer that 16-lane rows hold alike
 __device__ __forceinline__ int32_t row16_min(int32_t v) {
     v = min(v, dpp_i<DPP_XOR1>(v));
@@ -186,6 +211,7 @@ struct Tile {
 template <int TY, int D>
 struct Frag {
     using G = Tile<TY, D>;
+    static constexpr int PRE = 0;
     uint4 k[G::KR][G::KC];
     uint32_t v[G::VR][G::VW];
 
@@ -294,49 +320,23 @@ struct Wave16 {
                 for (int n = 0; n < NT; n++) q[n][c] = make_uint4(w[0][n], w[1][n], w[2][n], w[3][n]);
             }
         }
-        sc.cap = a.softcap * LOG2E;
-        sc.mul = a.softcap != 0.0f ? mul / a.softcap : mul * LOG2E;
-        sc.slope = a.slopes && r.valid ? a.slopes[r.head] * LOG2E : 0.0f;
-        sc.bare = a.softcap == 0.0f && !a.slopes && !__any(!(sc.mul > 0.0f));
+        sc = make_score(a, r, mul);
         m = NEG_INF;
         l = 0.0f;
 #pragma unroll
         for (int t = 0; t < G::DPL; t++) o[t] = f32x4{0, 0, 0, 0};
     }
 
-    // keys j0 .. j0 + KT of one tile, those from `end` on not of its segment;
-    // whole: every row sees all of them
-    template <class Src>
-    __device__ __forceinline__ void step(const Src &f, const Row &row, int32_t j0, int32_t end, bool whole, int lane) {
+    // The weights of one tile from its products, and the running maximum and sum; keys
+    // from `end` on are not of its segment; whole: the row sees all of them.
+    __device__ __forceinline__ void weights(float (&y)[G::VR], const Row &row, int32_t j0, int32_t end, bool whole,
+                                            int lane) {
         const int32_t g4 = 4 * (lane >> 4);
-        float y[G::VR];
-#pragma unroll
-        for (int t = 0; t < G::KR; t++) {
-            f32x4 s = {0, 0, 0, 0};
-#pragma unroll
-            for (int c = 0; c < G::KC; c++) {
-                const uint4 k = f.key(t, c);
-                if constexpr (TY == ATTN_F32) {
-                    const f32x4 kv = bits<f32x4>(k), qv = bits<f32x4>(q[0][c]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[i], qv[i], s, 0, 0, 0);
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NT; n++) s = mfma32<TY>(k, q[n][c], s);
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++) y[4 * t + r] = s[r];
-        }
         // with neither cap nor bias the product's factor goes into the exponent's
         // multiply-add, and y stays the bare product
         float mul = 1.0f;
-        if (sc.bare) {
-            mul = sc.mul;
-        } else {
-#pragma unroll
-            for (int r = 0; r < G::VR; r++) y[r] = score(sc, y[r], row.pos, j0 + 16 * (r >> 2) + g4 + (r & 3));
-        }
+        if (sc.bare) mul = sc.mul;
+        else scores(sc, y, row.pos - j0 - g4, [](int r) { return 16 * (r >> 2) + (r & 3); });
         if (!whole) {
             const int32_t hi = min(row.hi, end);
 #pragma unroll
@@ -361,29 +361,10 @@ struct Wave16 {
         }
         // fp16 terms of p stand 2^7 higher, so that the second ones stay normal
         const float base = (m == NEG_INF ? 0.0f : m) - (TY == ATTN_F16 ? 7.0f : 0.0f);
-        float p[G::VR];
 #pragma unroll
         for (int r = 0; r < G::VR; r++) {
-            p[r] = exp2_hw(fmaf(y[r], mul, -base));
-            l += p[r];
-        }
-        if constexpr (TY == ATTN_F32) {
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int t = 0; t < G::DPL; t++)
-                    o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.value(r, t), p[r], o[t], 0, 0, 0);
-        } else {
-            uint32_t pt[4][NT];
-#pragma unroll
-            for (int i = 0; i < 4; i++) split<TY>(p[2 * i], p[2 * i + 1], pt[i]);
-#pragma unroll
-            for (int t = 0; t < G::DPL; t++) {
-                const uint4 vt = f.value(t);
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-                    o[t] = mfma32<TY>(vt, make_uint4(pt[0][n], pt[1][n], pt[2][n], pt[3][n]), o[t]);
-            }
+            y[r] = exp2_hw(fmaf(y[r], mul, -base));
+            l += y[r];
         }
     }
 
@@ -397,6 +378,79 @@ struct Wave16 {
         return !(z == 0.0f);
     }
 };
+
+// One tile of keys for a wave's B blocks of 16 rows: every operand piece of K
+// and V is taken once for all of them.
+template <int TY, int D, int B, class Src>
+__device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Src &f, const Row (&row)[B], int32_t j0,
+                                          int32_t end, const bool (&whole)[B], int lane) {
+    using G = Tile<TY, D>;
+    constexpr int NT = TERMS<TY>;
+    float y[B][G::VR];
+#pragma unroll
+    for (int t = 0; t < G::KR; t++) {
+        f32x4 s[B];
+#pragma unroll
+        for (int b = 0; b < B; b++) s[b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < G::KC; c++) {
+            const uint4 k = f.key(t, c);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+                    if constexpr (TY == ATTN_F32) {
+                        const f32x4 kv = bits<f32x4>(k), qv = bits<f32x4>(st[b].q[0][c]);
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[i], qv[i], s[b], 0, 0, 0);
+                    } else {
+                        s[b] = mfma32<TY>(k, st[b].q[n][c], s[b]);
+                    }
+                }
+        }
+#pragma unroll
+        for (int b = 0; b < B; b++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[b][4 * t + r] = s[b][r];
+    }
+    // the first pieces of V are on their way while the weights are formed
+    constexpr int PRE = Src::PRE;
+    uint4 pre[PRE ? PRE : 1];
+    if constexpr (PRE) {
+#pragma unroll
+        for (int t = 0; t < PRE; t++) pre[t] = f.value(t);
+        asm volatile("" ::: "memory");
+    }
+#pragma unroll
+    for (int b = 0; b < B; b++) st[b].weights(y[b], row[b], j0, end, whole[b], lane);
+    if constexpr (TY == ATTN_F32) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int t = 0; t < G::DPL; t++) {
+                const float v = f.value(r, t);
+#pragma unroll
+                for (int b = 0; b < B; b++)
+                    st[b].o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, y[b][r], st[b].o[t], 0, 0, 0);
+            }
+    } else {
+        uint32_t pt[B][4][NT];
+#pragma unroll
+        for (int b = 0; b < B; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) split<TY>(y[b][2 * i], y[b][2 * i + 1], pt[b][i]);
+#pragma unroll
+        for (int t = 0; t < G::DPL; t++) {
+            const uint4 vt = t < PRE ? pre[t < PRE ? t : 0] : f.value(t);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int b = 0; b < B; b++)
+                    st[b].o[t] = mfma32<TY>(vt, make_uint4(pt[b][0][n], pt[b][1][n], pt[b][2][n], pt[b][3][n]), st[b].o[t]);
+        }
+    }
+}
 
 // Keys [c0, c1) of one segment: the shared prefix or a sequence's own cache.
 struct Segment {
@@ -437,11 +491,7 @@ __device__ __forceinline__ void row_again(const AttnArgs &a, uint32_t kvh, uint3
                                           int32_t c1, int wave, int lane, float (&acc)[D / 64], float &m, float &l) {
     using G = Tile<TY, D>;
     const float *qp = a.q + ((uint64_t)(uint32_t)r.row * a.n_head + r.head) * D;
-    Score sc;
-    sc.cap = a.softcap * LOG2E;
-    sc.mul = a.softcap != 0.0f ? a.scale / a.softcap : a.scale * LOG2E;
-    sc.slope = a.slopes ? a.slopes[r.head] * LOG2E : 0.0f;
-    sc.bare = false;
+    const Score sc = make_score(a, r, a.scale);
     m = NEG_INF;
     l = 0.0f;
 #pragma unroll
@@ -455,7 +505,9 @@ __device__ __forceinline__ void row_again(const AttnArgs &a, uint32_t kvh, uint3
 #pragma unroll
                 for (int e = 0; e < D / 64; e++)
                     d = fmaf(qp[lane + 64 * e], ld_kv<TY>(g.k + at, lane + 64 * e), d);
-                const float y = score(sc, group_sum<64>(d), r.pos, j);
+                float yj[1] = {group_sum<64>(d)};
+                scores(sc, yj, r.pos - j, [](int) { return 0; });
+                const float y = yj[0];
                 const float mn = y > m ? y : m;
                 const float f0 = m == NEG_INF ? 0.0f : exp2_hw(m - mn);
                 const float p = exp2_hw(y - (mn == NEG_INF ? 0.0f : mn));
@@ -593,12 +645,13 @@ __global__ void __launch_bounds__(256, D <= (TY == ATTN_BF16 ? 64 : 128) ? 2 : 1
     const Item it = make_item(a, blockIdx.x);
     SeqRows sr;
     const int32_t n_row = item_rows(a, it, sr);
-    const Row row = make_row(a, it.kvh, it.tile * 16 + (lane & 15), it.pooled, it.seq, sr, n_row);
+    const Row rows[1] = {make_row(a, it.kvh, it.tile * 16 + (lane & 15), it.pooled, it.seq, sr, n_row)};
+    const Row &row = rows[0];
     const Span sp = wave_span(a, it, sr, row);
     int32_t c0, c1;
     split_share(a, it, sp.lo, sp.hi, G::KT, c0, c1);
 
-    Wave16<TY, D> st;
+    Wave16<TY, D> sts[1], &st = sts[0];
     st.init(a, row, lane);
     for (int sg = 0; sg < 2; sg++) {
         const Segment g = segment(a, G::EB, it.kvh, it.seq, sg == 0, c0, c1);
@@ -608,14 +661,14 @@ __global__ void __launch_bounds__(256, D <= (TY == ATTN_BF16 ? 64 : 128) ? 2 : 1
         f.load(g.k, g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
         while (true) {
             const int32_t jn = j + W * G::KT;
-            const bool whole = j >= sp.all_lo && j + G::KT <= min(sp.all_hi, g.c1);
+            const bool whole[1] = {j >= sp.all_lo && j + G::KT <= min(sp.all_hi, g.c1)};
             if constexpr (D <= 128) {
                 Frag<TY, D> fn;
                 if (jn < g.c1) fn.load(g.k, g.v, g.row_bytes, jn - g.origin, g.c1 - g.origin, lane);
-                st.step(f, row, j, g.c1, whole, lane);
+                attn_step<TY, D, 1>(sts, f, rows, j, g.c1, whole, lane);
                 f = fn;
             } else {
-                st.step(f, row, j, g.c1, whole, lane);
+                attn_step<TY, D, 1>(sts, f, rows, j, g.c1, whole, lane);
                 if (jn < g.c1) f.load(g.k, g.v, g.row_bytes, jn - g.origin, g.c1 - g.origin, lane);
             }
             j = jn;
@@ -684,7 +737,7 @@ __global__ void __launch_bounds__(256, D <= (TY == ATTN_BF16 ? 64 : 128) ? 2 : 1
 template <int TY, int D, int NTHREADS>
 struct Stage {
     using G = Tile<TY, D>;
-    static constexpr int NK = TY == ATTN_F32 || (TY == ATTN_BF16 && D == 256) ? 32 : 64;   // 32: registers
+    static constexpr int NK = TY == ATTN_F32 || (TY == ATTN_BF16 && D == 256) || (TY == ATTN_F16 && D == 128) ? 32 : 64;   // 32: registers
     static constexpr int KROW = D * G::EB + 16, VBYTES = TY == ATTN_F32 ? NK * KROW : NK * D * 2;
     static constexpr int BYTES = NK * KROW + VBYTES;
     static constexpr int PER_ROW = D * G::EB / 16;                            // 16-byte pieces of a row
@@ -756,6 +809,7 @@ struct Stage {
     }
     // the operands of one of its tiles, as Frag gives them
     struct View {
+        static constexpr int PRE = TY == ATTN_F32 || D == 256 ? 0 : 4;
         const char *kp, *vp;
         __device__ __forceinline__ uint4 key(int t, int i) const { return *(const uint4 *)(kp + t * 16 * KROW + i * 64); }
         __device__ __forceinline__ uint4 value(int t) const { return *(const uint4 *)(vp + t * 1024); }
@@ -771,28 +825,41 @@ struct Stage {
     }
 };
 
-// Many rows: eight waves of 16 rows each walk the same keys, staged through
-// LDS for all of them (two buffers: the next keys are on their way from memory
-// while these are worked on, one barrier per stage).
+// Many rows: the waves of a workgroup, 16 B rows each, walk the same keys,
+// staged through LDS for all of them (two buffers: the next keys are on their
+// way from memory while these are worked on, one barrier per stage).
 template <int TY, int D>
-__global__ void __launch_bounds__(512, 2) k_attn_tile(const AttnArgs a) {
+constexpr int TILE_BLOCKS = D == 256 || (TY == ATTN_BF16 && D == 128) ? 1 : 2;   // B: what a wave's registers hold
+constexpr int TILE_ROWS = 128;                  // of a workgroup
+template <int TY, int D>
+constexpr int TILE_THREADS = 64 * TILE_ROWS / 16 / TILE_BLOCKS<TY, D>;
+template <int TY, int D>
+__global__ void __launch_bounds__((TILE_THREADS<TY, D>), 2) k_attn_tile(const AttnArgs a) {
     using G = Tile<TY, D>;
-    constexpr int W = 8;
-    using S = Stage<TY, D, 64 * W>;
+    constexpr int B = TILE_BLOCKS<TY, D>, W = TILE_ROWS / 16 / B;
+    using S = Stage<TY, D, TILE_THREADS<TY, D>>;
     __shared__ __align__(16) char lds[2][S::BYTES];
     __shared__ int32_t span[2][W];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Item it = make_item(a, blockIdx.x);
     SeqRows sr;
     const int32_t n_row = item_rows(a, it, sr);
-    const Row row = make_row(a, it.kvh, (it.tile * W + wave) * 16 + (lane & 15), it.pooled, it.seq, sr, n_row);
-    const Span sp = wave_span(a, it, sr, row);
+    Row row[B];
+    Span sp[B];
+    int32_t lo = INT32_MAX, hi = 0, c0, c1;
+#pragma unroll
+    for (int b = 0; b < B; b++) {
+        row[b] = make_row(a, it.kvh, it.tile * TILE_ROWS + (wave * B + b) * 16 + (lane & 15), it.pooled, it.seq, sr, n_row);
+        sp[b] = wave_span(a, it, sr, row[b]);
+        lo = min(lo, sp[b].lo);
+        hi = max(hi, sp[b].hi);
+    }
+    const int32_t wave_lo = lo, wave_hi = hi;
     if (lane == 0) {
-        span[0][wave] = sp.lo;
-        span[1][wave] = sp.hi;
+        span[0][wave] = lo;
+        span[1][wave] = hi;
     }
     __syncthreads();
-    int32_t lo = INT32_MAX, hi = 0, c0, c1;
 #pragma unroll
     for (int w = 0; w < W; w++) {
         lo = min(lo, span[0][w]);
@@ -802,8 +869,9 @@ __global__ void __launch_bounds__(512, 2) k_attn_tile(const AttnArgs a) {
     hi = __builtin_amdgcn_readfirstlane(hi);
     split_share(a, it, lo, hi, S::NK, c0, c1);
 
-    Wave16<TY, D> st;
-    st.init(a, row, lane);
+    Wave16<TY, D> st[B];
+#pragma unroll
+    for (int b = 0; b < B; b++) st[b].init(a, row[b], lane);
     S stage;
     for (int sg = 0; sg < 2; sg++) {
         const Segment g = segment(a, G::EB, it.kvh, it.seq, sg == 0, c0, c1);
@@ -819,36 +887,40 @@ __global__ void __launch_bounds__(512, 2) k_attn_tile(const AttnArgs a) {
 #pragma unroll 1
             for (int sub = 0; sub < S::NK / G::KT; sub++) {
                 const int32_t js = j + sub * G::KT;
-                if (js >= min(sp.hi, g.c1) || js + G::KT <= sp.lo) continue;
-                const bool whole = js >= sp.all_lo && js + G::KT <= min(sp.all_hi, g.c1);
-                st.step(S::view(lds[at], sub, lane), row, js, g.c1, whole, lane);
+                if (js >= min(wave_hi, g.c1) || js + G::KT <= wave_lo) continue;
+                bool whole[B];
+#pragma unroll
+                for (int b = 0; b < B; b++) whole[b] = js >= sp[b].all_lo && js + G::KT <= min(sp[b].all_hi, g.c1);
+                attn_step<TY, D, B>(st, S::view(lds[at], sub, lane), row, js, g.c1, whole, lane);
             }
             if (more) stage.store(lds[at ^ 1]);
             __syncthreads();
             at ^= 1;
         }
     }
-    st.l = rows_sum(st.l);
-    odd_rows<TY, D, 1>(a, it, row, c0, c1, 0, lane, st, (float *)lds[0] + wave * D);
-
-    if (!row.valid) return;
-    float *dst;
-    float f0 = 1.0f;
-    if (a.slots) {
-        const uint64_t at = slot_of(a, row_head(a, row), it);
-        if (lane < 16) a.ml[at] = make_float2(st.m, st.l);
-        dst = a.acc + at * D;
-        if (st.l == 0.0f) return;
-    } else {
-        f0 = st.l == 0.0f ? 0.0f : 1.0f / st.l;
-        dst = a.out + row_head(a, row) * D;
+#pragma unroll
+    for (int b = 0; b < B; b++) {
+        st[b].l = rows_sum(st[b].l);
+        odd_rows<TY, D, 1>(a, it, row[b], c0, c1, 0, lane, st[b], (float *)lds[0] + wave * D);
+        if (!row[b].valid) continue;
+        float *dst;
+        float f0 = 1.0f;
+        if (a.slots) {
+            const uint64_t at = slot_of(a, row_head(a, row[b]), it);
+            if (lane < 16) a.ml[at] = make_float2(st[b].m, st[b].l);
+            dst = a.acc + at * D;
+            if (st[b].l == 0.0f) continue;
+        } else {
+            f0 = st[b].l == 0.0f ? 0.0f : 1.0f / st[b].l;
+            dst = a.out + row_head(a, row[b]) * D;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int t = 0; t < G::DPL; t += 4)
+                *(float4 *)(dst + G::DPL * (4 * (lane >> 4) + q) + t) = make_float4(
+                    st[b].o[t][q] * f0, st[b].o[t + 1][q] * f0, st[b].o[t + 2][q] * f0, st[b].o[t + 3][q] * f0);
     }
-#pragma unroll
-    for (int q = 0; q < 4; q++)
-#pragma unroll
-        for (int t = 0; t < G::DPL; t += 4)
-            *(float4 *)(dst + G::DPL * (4 * (lane >> 4) + q) + t) =
-                make_float4(st.o[t][q] * f0, st.o[t + 1][q] * f0, st.o[t + 2][q] * f0, st.o[t + 3][q] * f0);
 }
 
 // The partial sums of a row, joined: one wave per (row, head).
@@ -885,7 +957,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
 
 template <int TY, int D>
 static hipError_t attn_run(const AttnArgs &a, bool rows, uint32_t items, hipStream_t s) {
-    if (rows) hipLaunchKernelGGL((k_attn_tile<TY, D>), dim3(items), dim3(512), 0, s, a);
+    if (rows) hipLaunchKernelGGL((k_attn_tile<TY, D>), dim3(items), dim3(TILE_THREADS<TY, D>), 0, s, a);
     else hipLaunchKernelGGL((k_attn<TY, D>), dim3(items), dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !a.slots) return e;
