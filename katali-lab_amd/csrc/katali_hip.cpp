@@ -532,7 +532,7 @@ int attn_impl(const KataliHipAttn *a, const KataliHipAttnPrefix *p, const float 
         g.n_shared = p->n_prefix;
     }
     const kq::AttnPlan plan = kq::attn_plan(g.n_seq, g.n_rows, g.max_q, g.n_kv, g.group, g.max_kv, g.n_shared,
-                                            a->head_dim, (uint32_t)kq::device_cu_count());
+                                            a->head_dim, (int)a->kv_type, (uint32_t)kq::device_cu_count());
     return launched(kq::launch_attn(g, a->kv_type, a->head_dim, plan, g_attn, g_stream), "attention");
 }
 

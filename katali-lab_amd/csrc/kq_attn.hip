@@ -589,7 +589,8 @@ __device__ __forceinline__ void split_share(const AttnArgs &a, const Item &it, i
     c0 = c1 = 0;
     if (hi <= lo) return;
     const uint32_t n = (uint32_t)(hi - lo), splits = it.pooled ? a.shared_splits : a.own_splits;
-    const uint32_t used = min(max((n + a.min_chunk - 1) / a.min_chunk, 1u), splits);
+    const uint32_t worth = it.pooled ? a.shared_chunk : a.own_chunk;
+    const uint32_t used = min((n + worth - 1) / worth, splits);
     const uint32_t chunk = ((n + used - 1) / used + tile - 1) / tile * tile;
     const uint64_t b = (uint64_t)it.split * chunk;
     if (b < n) {
@@ -632,17 +633,24 @@ __device__ __forceinline__ void odd_rows(const AttnArgs &a, const Item &it, cons
     }
 }
 
-// Few rows: the four waves of a workgroup share 16 rows and take every fourth tile of the keys.
-template <int TY, int D>
-__global__ void __launch_bounds__(256, D <= (TY == ATTN_BF16 ? 64 : 128) ? 2 : 1) k_attn(const AttnArgs a) {
+// Few rows: the waves of a workgroup share 16 rows and take every W-th tile of
+// the keys, straight from memory into the operands' registers, the next tile's
+// on their way while one is worked on (where the registers hold two; with
+// 256-wide heads, and 128-wide ones of bf16 with their third terms, they do not,
+// and the waves cover for each other).
+constexpr int ROWS_WAVES = 4;
+template <int TY, int D, int W>
+struct RowsLds {
+    float o[W][16][D + 4];
+    float m[W][16], l[W][16];
+    uint64_t at[16];   // packed row x head of each row, ~0 for none
+};
+template <int TY, int D, int W>
+__device__ __forceinline__ void attn_rows_item(const AttnArgs &a, const Item &it, char *shared) {
     using G = Tile<TY, D>;
-    constexpr int W = 4;
-    __shared__ float lds_o[W][16][D + 4];
-    __shared__ float lds_m[W][16], lds_l[W][16];
-    __shared__ float lds_row[W][D];
-    __shared__ uint64_t lds_at[16];   // packed row x head of each tile row, ~0 for none
+    constexpr bool AHEAD = D == 64 || (D == 128 && TY != ATTN_BF16);
+    auto &lds = *(RowsLds<TY, D, W> *)shared;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Item it = make_item(a, blockIdx.x);
     SeqRows sr;
     const int32_t n_row = item_rows(a, it, sr);
     const Row rows[1] = {make_row(a, it.kvh, it.tile * 16 + (lane & 15), it.pooled, it.seq, sr, n_row)};
@@ -651,63 +659,76 @@ __global__ void __launch_bounds__(256, D <= (TY == ATTN_BF16 ? 64 : 128) ? 2 : 1
     int32_t c0, c1;
     split_share(a, it, sp.lo, sp.hi, G::KT, c0, c1);
 
+    // the wave's first tile is asked for before q is waited for
+    Segment g = segment(a, G::EB, it.kvh, it.seq, true, c0, c1);
+    int32_t j = g.c0 + wave * G::KT;
+    bool own = false;
+    if (j >= g.c1) {
+        g = segment(a, G::EB, it.kvh, it.seq, false, c0, c1);
+        j = g.c0 + wave * G::KT;
+        own = true;
+    }
+    Frag<TY, D> f;
+    bool some = j < g.c1;
+    if (some) f.load(g.k, g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
     Wave16<TY, D> sts[1], &st = sts[0];
     st.init(a, row, lane);
-    for (int sg = 0; sg < 2; sg++) {
-        const Segment g = segment(a, G::EB, it.kvh, it.seq, sg == 0, c0, c1);
-        int32_t j = g.c0 + wave * G::KT;
-        if (j >= g.c1) continue;
-        Frag<TY, D> f;
-        f.load(g.k, g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
-        while (true) {
-            const int32_t jn = j + W * G::KT;
-            const bool whole[1] = {j >= sp.all_lo && j + G::KT <= min(sp.all_hi, g.c1)};
-            if constexpr (D <= 128) {
-                Frag<TY, D> fn;
-                if (jn < g.c1) fn.load(g.k, g.v, g.row_bytes, jn - g.origin, g.c1 - g.origin, lane);
-                attn_step<TY, D, 1>(sts, f, rows, j, g.c1, whole, lane);
-                f = fn;
-            } else {
-                attn_step<TY, D, 1>(sts, f, rows, j, g.c1, whole, lane);
-                if (jn < g.c1) f.load(g.k, g.v, g.row_bytes, jn - g.origin, g.c1 - g.origin, lane);
-            }
-            j = jn;
-            if (j >= g.c1) break;
+    while (some) {
+        Segment gn = g;
+        int32_t jn = j + W * G::KT;
+        if (jn >= g.c1 && !own) {
+            gn = segment(a, G::EB, it.kvh, it.seq, false, c0, c1);
+            jn = gn.c0 + wave * G::KT;
+            own = true;
         }
+        const bool more = jn < gn.c1;
+        const bool whole[1] = {j >= sp.all_lo && j + G::KT <= min(sp.all_hi, g.c1)};
+        if constexpr (AHEAD) {
+            Frag<TY, D> fn;
+            if (more) fn.load(gn.k, gn.v, gn.row_bytes, jn - gn.origin, gn.c1 - gn.origin, lane);
+            attn_step<TY, D, 1>(sts, f, rows, j, g.c1, whole, lane);
+            f = fn;
+        } else {
+            attn_step<TY, D, 1>(sts, f, rows, j, g.c1, whole, lane);
+            if (more) f.load(gn.k, gn.v, gn.row_bytes, jn - gn.origin, gn.c1 - gn.origin, lane);
+        }
+        g = gn;
+        j = jn;
+        some = more;
     }
     st.l = rows_sum(st.l);
-    odd_rows<TY, D, W>(a, it, row, c0, c1, wave, lane, st, lds_row[wave]);
+    odd_rows<TY, D, W>(a, it, row, c0, c1, wave, lane, st, &lds.o[wave][0][0]);
 
-    // the four waves' sums of the same rows, joined in LDS
+    // the waves' sums of the same rows, joined in LDS
     if (lane < 16) {
-        lds_m[wave][lane] = st.m;
-        lds_l[wave][lane] = st.l;
-        if (wave == 0) lds_at[lane] = row.valid ? row_head(a, row) : ~0ull;
+        lds.m[wave][lane] = st.m;
+        lds.l[wave][lane] = st.l;
+        if (wave == 0) lds.at[lane] = row.valid ? row_head(a, row) : ~0ull;
     }
 #pragma unroll
     for (int q = 0; q < 4; q++)
 #pragma unroll
         for (int t = 0; t < G::DPL; t += 4)
-            *(float4 *)&lds_o[wave][lane & 15][G::DPL * (4 * (lane >> 4) + q) + t] =
+            *(float4 *)&lds.o[wave][lane & 15][G::DPL * (4 * (lane >> 4) + q) + t] =
                 make_float4(st.o[t][q], st.o[t + 1][q], st.o[t + 2][q], st.o[t + 3][q]);
     __syncthreads();
-    // thread: row tid / 16, columns D/16 (tid % 16) ...
-    const int i = threadIdx.x >> 4;
-    const uint64_t rh = lds_at[i];
+    // thread: row tid / (4 W), columns 4 (tid % (4 W)), + 16 W, ...
+    const int i = threadIdx.x / (4 * W);
+    const uint64_t rh = lds.at[i];
     if (rh == ~0ull) return;
     float m = NEG_INF, l = 0.0f, w[W];
 #pragma unroll
-    for (int k = 0; k < W; k++) m = fmaxf(m, lds_m[k][i]);
+    for (int k = 0; k < W; k++) m = fmaxf(m, lds.m[k][i]);
 #pragma unroll
     for (int k = 0; k < W; k++) {
-        w[k] = lds_l[k][i] == 0.0f ? 0.0f : exp2_hw(lds_m[k][i] - m);
-        l += lds_l[k][i] * w[k];
+        w[k] = lds.l[k][i] == 0.0f ? 0.0f : exp2_hw(lds.m[k][i] - m);
+        l += lds.l[k][i] * w[k];
     }
     float *dst;
     float f0 = 1.0f;
     if (a.slots) {
         const uint64_t at = slot_of(a, rh, it);
-        if ((threadIdx.x & 15) == 0) a.ml[at] = make_float2(m, l);
+        if (threadIdx.x % (4 * W) == 0) a.ml[at] = make_float2(m, l);
         if (l == 0.0f) return;
         dst = a.acc + at * D;
     } else {
@@ -715,14 +736,17 @@ __global__ void __launch_bounds__(256, D <= (TY == ATTN_BF16 ? 64 : 128) ? 2 : 1
         dst = a.out + rh * D;
     }
 #pragma unroll
-    for (int t = 0; t < G::DPL; t += 4) {
-        const int col = (threadIdx.x & 15) * G::DPL + t;
+    for (int c = 0; c < D; c += 16 * W) {
+        const int col = c + threadIdx.x % (4 * W) * 4;
+        if (col >= D) break;
         float x[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < W; k++) {
+            const float4 v = *(const float4 *)&lds.o[k][i][col];
+            const float e[4] = {v.x, v.y, v.z, v.w};
             if (w[k] == 0.0f) continue;
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = fmaf(lds_o[k][i][col + e], w[k], x[e]);
+            for (int n = 0; n < 4; n++) x[n] = fmaf(e[n], w[k], x[n]);
         }
         *(float4 *)(dst + col) = make_float4(x[0] * f0, x[1] * f0, x[2] * f0, x[3] * f0);
     }
@@ -828,20 +852,18 @@ struct Stage {
 // Many rows: the waves of a workgroup, 16 B rows each, walk the same keys,
 // staged through LDS for all of them (two buffers: the next keys are on their
 // way from memory while these are worked on, one barrier per stage).
-template <int TY, int D>
-constexpr int TILE_BLOCKS = D == 256 || (TY == ATTN_BF16 && D == 128) ? 1 : 2;   // B: what a wave's registers hold
-constexpr int TILE_ROWS = 128;                  // of a workgroup
-template <int TY, int D>
-constexpr int TILE_THREADS = 64 * TILE_ROWS / 16 / TILE_BLOCKS<TY, D>;
-template <int TY, int D>
-__global__ void __launch_bounds__((TILE_THREADS<TY, D>), 2) k_attn_tile(const AttnArgs a) {
+template <int TY, int D, int B, int W>
+struct TileLds {
+    char stage[2][Stage<TY, D, 64 * W>::BYTES];
+    int32_t span[2][W];
+};
+template <int TY, int D, int B, int W>
+__device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it, char *shared) {
     using G = Tile<TY, D>;
-    constexpr int B = TILE_BLOCKS<TY, D>, W = TILE_ROWS / 16 / B;
-    using S = Stage<TY, D, TILE_THREADS<TY, D>>;
-    __shared__ __align__(16) char lds[2][S::BYTES];
-    __shared__ int32_t span[2][W];
+    using S = Stage<TY, D, 64 * W>;
+    constexpr int ROWS = 16 * B * W;
+    auto &lds = *(TileLds<TY, D, B, W> *)shared;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Item it = make_item(a, blockIdx.x);
     SeqRows sr;
     const int32_t n_row = item_rows(a, it, sr);
     Row row[B];
@@ -849,21 +871,21 @@ __global__ void __launch_bounds__((TILE_THREADS<TY, D>), 2) k_attn_tile(const At
     int32_t lo = INT32_MAX, hi = 0, c0, c1;
 #pragma unroll
     for (int b = 0; b < B; b++) {
-        row[b] = make_row(a, it.kvh, it.tile * TILE_ROWS + (wave * B + b) * 16 + (lane & 15), it.pooled, it.seq, sr, n_row);
+        row[b] = make_row(a, it.kvh, it.tile * ROWS + (wave * B + b) * 16 + (lane & 15), it.pooled, it.seq, sr, n_row);
         sp[b] = wave_span(a, it, sr, row[b]);
         lo = min(lo, sp[b].lo);
         hi = max(hi, sp[b].hi);
     }
     const int32_t wave_lo = lo, wave_hi = hi;
     if (lane == 0) {
-        span[0][wave] = lo;
-        span[1][wave] = hi;
+        lds.span[0][wave] = lo;
+        lds.span[1][wave] = hi;
     }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < W; w++) {
-        lo = min(lo, span[0][w]);
-        hi = max(hi, span[1][w]);
+        lo = min(lo, lds.span[0][w]);
+        hi = max(hi, lds.span[1][w]);
     }
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
@@ -879,7 +901,7 @@ __global__ void __launch_bounds__((TILE_THREADS<TY, D>), 2) k_attn_tile(const At
         stage.fetch(g.k, g.v, g.row_bytes, g.c0 - g.origin, g.c1 - g.origin);
         int at = 0;
         __syncthreads();   // the last segment's readers are done
-        stage.store(lds[0]);
+        stage.store(lds.stage[0]);
         __syncthreads();
         for (int32_t j = g.c0; j < g.c1; j += S::NK) {
             const bool more = j + S::NK < g.c1;
@@ -891,9 +913,9 @@ __global__ void __launch_bounds__((TILE_THREADS<TY, D>), 2) k_attn_tile(const At
                 bool whole[B];
 #pragma unroll
                 for (int b = 0; b < B; b++) whole[b] = js >= sp[b].all_lo && js + G::KT <= min(sp[b].all_hi, g.c1);
-                attn_step<TY, D, B>(st, S::view(lds[at], sub, lane), row, js, g.c1, whole, lane);
+                attn_step<TY, D, B>(st, S::view(lds.stage[at], sub, lane), row, js, g.c1, whole, lane);
             }
-            if (more) stage.store(lds[at ^ 1]);
+            if (more) stage.store(lds.stage[at ^ 1]);
             __syncthreads();
             at ^= 1;
         }
@@ -901,7 +923,7 @@ __global__ void __launch_bounds__((TILE_THREADS<TY, D>), 2) k_attn_tile(const At
 #pragma unroll
     for (int b = 0; b < B; b++) {
         st[b].l = rows_sum(st[b].l);
-        odd_rows<TY, D, 1>(a, it, row[b], c0, c1, 0, lane, st[b], (float *)lds[0] + wave * D);
+        odd_rows<TY, D, 1>(a, it, row[b], c0, c1, 0, lane, st[b], (float *)lds.stage[0] + wave * D);
         if (!row[b].valid) continue;
         float *dst;
         float f0 = 1.0f;
@@ -923,13 +945,43 @@ __global__ void __launch_bounds__((TILE_THREADS<TY, D>), 2) k_attn_tile(const At
     }
 }
 
-// The partial sums of a row, joined: one wave per (row, head).
-template <int D>
+// The kernels. Mixed: a batch's shared prefix for the rows of all sequences
+// together (many rows) beside each sequence's own keys (few rows), in one
+// launch, so that matrix work and memory traffic overlap.
+template <int TY, int D>
+__global__ void __launch_bounds__(64 * ROWS_WAVES, D == 256 ? 1 : 2) k_attn(const AttnArgs a) {
+    __shared__ __align__(16) char lds[sizeof(RowsLds<TY, D, ROWS_WAVES>)];
+    attn_rows_item<TY, D, ROWS_WAVES>(a, make_item(a, blockIdx.x), lds);
+}
+// (eight waves where four would need more registers to stage the keys than there are)
+template <int TY, int D>
+constexpr int TILE_WAVES = TY == ATTN_BF16 && D == 256 ? 8 : 4;
+template <int TY, int D>
+__global__ void __launch_bounds__((64 * TILE_WAVES<TY, D>), 2) k_attn_tile(const AttnArgs a) {
+    constexpr int W = TILE_WAVES<TY, D>, B = attn_tile_rows(TY, D) / (16 * W);
+    __shared__ __align__(16) char lds[sizeof(TileLds<TY, D, B, W>)];
+    attn_tile_item<TY, D, B, W>(a, make_item(a, blockIdx.x), lds);
+}
+template <int TY, int D>
+__global__ void __launch_bounds__(64 * ROWS_WAVES, D == 256 ? 1 : 2) k_attn_mixed(const AttnArgs a) {
+    constexpr int W = ROWS_WAVES;
+    constexpr size_t R = sizeof(RowsLds<TY, D, W>), T = sizeof(TileLds<TY, D, 1, W>);
+    __shared__ __align__(16) char lds[R > T ? R : T];
+    const Item it = make_item(a, blockIdx.x);
+    if (it.pooled) attn_tile_item<TY, D, 1, W>(a, it, lds);
+    else attn_rows_item<TY, D, W>(a, it, lds);
+}
+
+// The partial sums of a row, joined: SW waves per (row, head), each every
+// SW-th slot, eight slots' loads in flight.
+template <int D, int SW>
 __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
-    const int lane = threadIdx.x & 63;
-    const uint32_t heads4 = (a.n_head + 3) / 4;
-    const uint32_t head = blockIdx.x % heads4 * 4 + (threadIdx.x >> 6);
-    const uint32_t id = blockIdx.x / heads4, seq = id / a.max_q, t = id % a.max_q;
+    constexpr int E = D / 64, U = 8;
+    __shared__ float part[SW > 1 ? SW : 1][SW > 1 ? D : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t per = 4 / SW, blocks = (a.n_head + per - 1) / per;
+    const uint32_t head = blockIdx.x % blocks * per + wave / SW;
+    const uint32_t id = blockIdx.x / blocks, seq = id / a.max_q, t = id % a.max_q;
     const SeqRows sr = seq_rows(a, seq);
     if (head >= a.n_head || (int32_t)t >= sr.last - sr.first) return;
     const uint64_t rh = (uint64_t)(uint32_t)(sr.first + (int32_t)t) * a.n_head + head;
@@ -941,27 +993,51 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
     const float w = ml.y == 0.0f ? 0.0f : exp2_hw(ml.x - m);
     const float l = group_sum<64>(ml.y * w);
     const float f0 = l == 0.0f ? 0.0f : 1.0f / l;
-    float x[D / 64];
+    float x[E];
 #pragma unroll
-    for (int e = 0; e < D / 64; e++) x[e] = 0.0f;
-    for (uint32_t k = 0; k < a.slots; k++) {
-        const float wk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), k));
-        if (wk == 0.0f) continue;
-        const float *p = a.acc + (rh * a.slots + k) * D;
+    for (int e = 0; e < E; e++) x[e] = 0.0f;
+    const float *p = a.acc + rh * a.slots * D + lane;
+    for (uint32_t k0 = wave % SW; k0 < a.slots; k0 += SW * U) {
+        float v[U][E];
 #pragma unroll
-        for (int e = 0; e < D / 64; e++) x[e] = fmaf(p[lane + 64 * e], wk, x[e]);
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < E; e++) v[u][e] = p[(uint64_t)min(k0 + SW * u, a.slots - 1) * D + 64 * e];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t k = k0 + SW * u;
+            const float wk = k < a.slots ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), k & 63)) : 0.0f;
+            // a slot that weighs nothing may hold anything
+#pragma unroll
+            for (int e = 0; e < E; e++) x[e] = wk == 0.0f ? x[e] : fmaf(v[u][e], wk, x[e]);
+        }
+    }
+    if constexpr (SW > 1) {
+#pragma unroll
+        for (int e = 0; e < E; e++) part[wave][lane + 64 * e] = x[e];
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int e = 0; e < E; e++)
+#pragma unroll
+            for (int k = 1; k < SW; k++) x[e] += part[k][lane + 64 * e];
     }
 #pragma unroll
-    for (int e = 0; e < D / 64; e++) a.out[rh * D + lane + 64 * e] = x[e] * f0;
+    for (int e = 0; e < E; e++) a.out[rh * D + lane + 64 * e] = x[e] * f0;
 }
 
 template <int TY, int D>
-static hipError_t attn_run(const AttnArgs &a, bool rows, uint32_t items, hipStream_t s) {
-    if (rows) hipLaunchKernelGGL((k_attn_tile<TY, D>), dim3(items), dim3(TILE_THREADS<TY, D>), 0, s, a);
-    else hipLaunchKernelGGL((k_attn<TY, D>), dim3(items), dim3(256), 0, s, a);
+static hipError_t attn_run(const AttnArgs &a, AttnForm form, uint32_t items, hipStream_t s) {
+    const dim3 g(items);
+    if (form == ATTN_TILES) hipLaunchKernelGGL((k_attn_tile<TY, D>), g, dim3(64 * TILE_WAVES<TY, D>), 0, s, a);
+    else if (form == ATTN_MIXED) hipLaunchKernelGGL((k_attn_mixed<TY, D>), g, dim3(64 * ROWS_WAVES), 0, s, a);
+    else hipLaunchKernelGGL((k_attn<TY, D>), g, dim3(64 * ROWS_WAVES), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !a.slots) return e;
-    hipLaunchKernelGGL((k_attn_join<D>), dim3(a.n_seq * a.max_q * ((a.n_head + 3) / 4)), dim3(256), 0, s, a);
+    // four waves a row where many slots meet and there are few rows
+    const uint32_t rows = a.n_seq * a.max_q;
+    if (a.slots > 8) hipLaunchKernelGGL((k_attn_join<D, 4>), dim3(rows * a.n_head), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_join<D, 1>), dim3(rows * ((a.n_head + 3) / 4)), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
@@ -972,15 +1048,16 @@ hipError_t launch_attn(AttnArgs a, uint32_t type, uint32_t head_dim, const AttnP
     a.shared_splits = p.shared_splits;
     a.slots = p.slots;
     a.own_items = p.own_items;
-    a.min_chunk = p.min_chunk;
+    a.own_chunk = p.own_chunk;
+    a.shared_chunk = p.shared_chunk;
     a.acc = (float *)scratch;
     a.ml = (float2 *)((char *)scratch + (uint64_t)a.n_rows * a.n_head * p.slots * head_dim * 4);
     const uint32_t items = p.own_items + p.shared_items;
     auto go = [&](auto ty) -> hipError_t {
         constexpr int TY = decltype(ty)::value;
-        if (head_dim == 64) return attn_run<TY, 64>(a, p.rows, items, s);
-        if (head_dim == 128) return attn_run<TY, 128>(a, p.rows, items, s);
-        return attn_run<TY, 256>(a, p.rows, items, s);
+        if (head_dim == 64) return attn_run<TY, 64>(a, p.form, items, s);
+        if (head_dim == 128) return attn_run<TY, 128>(a, p.form, items, s);
+        return attn_run<TY, 256>(a, p.form, items, s);
     };
     if (type == ATTN_F32) return go(std::integral_constant<int, ATTN_F32>());
     if (type == ATTN_F16) return go(std::integral_constant<int, ATTN_F16>());

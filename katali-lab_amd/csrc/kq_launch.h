@@ -296,7 +296,6 @@ uint64_t moe_route_words();
 
 // Attention over caches (kq_attn.hip) and the step that stores new rows
 // (kq_kv.hip). Strides in cache values; arrays as KataliHipAttn describes them.
-constexpr int ATTN_F32 = 0, ATTN_F16 = 1, ATTN_BF16 = 30;   // cache types (ggml ids)
 struct AttnArgs {
     const float *q;
     float *out;
@@ -308,7 +307,7 @@ struct AttnArgs {
     uint32_t causal;
     float scale, softcap;
     // the plan, set by launch_attn
-    uint32_t own_tiles, own_splits, shared_tiles, shared_splits, slots, own_items, min_chunk;
+    uint32_t own_tiles, own_splits, shared_tiles, shared_splits, slots, own_items, own_chunk, shared_chunk;
     float *acc;
     float2 *ml;
 };

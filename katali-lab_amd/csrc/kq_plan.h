@@ -72,50 +72,73 @@ inline bool down_plan(bool q6, uint32_t hidden, uint32_t ffn, uint32_t n_slots, 
     return true;
 }
 
-// How an attention call's rows and keys are spread over workgroups (k_attn).
-// The rows of one key head of a sequence (query rows x the heads that share
-// the key head) make tiles of 16; with `rows` a workgroup takes eight tiles,
-// else one. Keys are split where the tiles alone would leave CUs idle, into
-// parts of at least min_chunk keys; the parts' sums then meet in `slots`
-// partial results of each row. A shared prefix is either an item of its own
-// for the rows of all sequences together (shared_tiles > 0) or walked by each
-// sequence's items ahead of its own keys.
+// How an attention call's rows and keys are spread over workgroups. The rows
+// of one key head of a sequence (query rows x the heads that share the key
+// head) make tiles: of 16 where they are few (the waves of a workgroup share
+// the rows and divide the keys), else of 128, 16 or 32 to a wave, which walk
+// the same keys together. Keys are split where the tiles alone would leave
+// CUs idle; the parts' sums meet in `slots` partial results of each row
+// (0: one part, written as the output). A shared prefix is either an item of
+// its own for the rows of all sequences together (shared_tiles > 0), or
+// walked by each sequence's items ahead of its own keys.
+enum AttnForm { ATTN_ROWS, ATTN_TILES, ATTN_MIXED };   // MIXED: pooled rows in tiles, own ones few
 struct AttnPlan {
-    bool rows;
+    AttnForm form;
     uint32_t own_tiles, own_splits, own_items;
     uint32_t shared_tiles, shared_splits, shared_items;
-    uint32_t slots, min_chunk;
+    uint32_t slots, own_chunk, shared_chunk;   // chunk: keys that are worth a part of their own
 };
 constexpr uint32_t ATTN_MAX_SLOTS = 64;
 constexpr uint64_t ATTN_SCRATCH = 64ull << 20;   // partial results: head_dim sums, a maximum and a sum each
+constexpr uint32_t ATTN_FEW_ROWS = 32;           // rows of a key head up to which tiles of 16 are taken
+
+constexpr int ATTN_F32 = 0, ATTN_F16 = 1, ATTN_BF16 = 30;   // cache types (ggml ids)
+// Rows of a workgroup's tile: 16 for each of four waves (bf16, 256: eight), 32 where a wave's
+// registers hold two blocks and its products are not the bound by themselves (fp32's are).
+constexpr int attn_tile_rows(int type, int head_dim) {
+    return type == ATTN_F32 || (type == ATTN_F16 && head_dim == 256) || (type == ATTN_BF16 && head_dim == 128) ? 64 : 128;
+}
 
 inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint32_t n_kv, uint32_t group,
-                          uint32_t max_kv, uint32_t n_shared, uint32_t head_dim, uint32_t cus) {
+                          uint32_t max_kv, uint32_t n_shared, uint32_t head_dim, int type, uint32_t cus) {
+    const bool f32 = type == ATTN_F32;
     AttnPlan p = {};
     const uint64_t per_seq = (uint64_t)max_q * group, n_head = (uint64_t)n_kv * group;
     const uint64_t most_slots = ATTN_SCRATCH / ((uint64_t)n_rows * n_head * (head_dim + 2) * 4);
-    p.min_chunk = 128;
-    p.rows = per_seq > 32;
-    const uint32_t tile = p.rows ? 128 : 16;
-    p.own_tiles = (uint32_t)((per_seq + tile - 1) / tile);
-    auto splits = [&](uint64_t items, uint64_t keys, uint64_t most) -> uint32_t {
-        uint64_t n = 2ull * cus / (items ? items : 1);
-        n = n < (keys + p.min_chunk - 1) / p.min_chunk ? n : (keys + p.min_chunk - 1) / p.min_chunk;
+    const uint32_t cap = most_slots < ATTN_MAX_SLOTS ? (uint32_t)most_slots : ATTN_MAX_SLOTS;
+    const uint32_t waves = 4;                               // ROWS_WAVES
+    const uint32_t few = waves * (f32 ? 16 : 32);           // a tile of keys for every wave
+    const uint32_t many = f32 ? 128 : 256;                  // four to eight stages
+    auto cover = [](uint64_t n, uint64_t by) { return (n + by - 1) / by; };
+    // parts for `items` items of up to `keys` keys each, so that about `want` workgroups come of it;
+    // a part has at least `least` keys, and shorter items take fewer parts of the same length
+    auto split = [&](uint64_t items, uint64_t keys, uint64_t want, uint32_t least, uint32_t most, uint32_t &parts,
+                     uint32_t &chunk) {
+        uint64_t n = want / (items ? items : 1);
+        const uint64_t worth = cover(keys, least);
+        n = n < worth ? n : worth;
         n = n < most ? n : most;
-        return n < 1 ? 1 : (uint32_t)n;
+        parts = n < 1 ? 1 : (uint32_t)n;
+        const uint64_t c = cover(keys ? keys : 1, parts);
+        chunk = (uint32_t)(c > least ? c : least);
     };
-    const uint64_t own = (uint64_t)n_seq * n_kv * p.own_tiles;
-    const uint64_t cap = most_slots < ATTN_MAX_SLOTS ? most_slots : ATTN_MAX_SLOTS;
-    if (n_shared && n_seq > 1 && !p.rows && cap >= 2) {
-        p.shared_tiles = (uint32_t)(((uint64_t)n_rows * group + tile - 1) / tile);
-        p.shared_splits = splits((uint64_t)n_kv * p.shared_tiles, n_shared, cap / 2);
-        p.own_splits = splits(own, max_kv, cap - p.shared_splits);
+    const bool tiles = per_seq > ATTN_FEW_ROWS;
+    p.own_tiles = (uint32_t)cover(per_seq, tiles ? attn_tile_rows(type, (int)head_dim) : 16);
+    const uint64_t own = (uint64_t)p.own_tiles * n_seq * n_kv;
+    if (n_shared && n_seq > 1 && !tiles && cap >= 2) {
+        const uint64_t pooled = (uint64_t)n_rows * group;
+        p.form = pooled > ATTN_FEW_ROWS ? ATTN_MIXED : ATTN_ROWS;
+        p.shared_tiles = (uint32_t)cover(pooled, p.form == ATTN_MIXED ? 16 * waves : 16);
+        split((uint64_t)n_kv * p.shared_tiles, n_shared, 2 * cus, p.form == ATTN_MIXED ? many : few, cap / 2,
+              p.shared_splits, p.shared_chunk);
+        split(own, max_kv, 2 * cus, few, cap - p.shared_splits, p.own_splits, p.own_chunk);
         p.slots = p.shared_splits + p.own_splits;
     } else {
-        p.own_splits = splits(own, (uint64_t)max_kv + n_shared, cap);
+        p.form = tiles ? ATTN_TILES : ATTN_ROWS;
+        split(own, (uint64_t)max_kv + n_shared, 2 * cus, tiles ? many : few, cap, p.own_splits, p.own_chunk);
         p.slots = p.own_splits > 1 ? p.own_splits : 0;
     }
-    p.own_items = (uint32_t)own * p.own_splits;
+    p.own_items = (uint32_t)(own * p.own_splits);
     p.shared_items = n_kv * p.shared_tiles * p.shared_splits;
     return p;
 }
