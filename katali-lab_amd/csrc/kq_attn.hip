@@ -211,7 +211,7 @@ struct Tile {
 template <int TY, int D>
 struct Frag {
     using G = Tile<TY, D>;
-    static constexpr int PRE = 0;
+    static constexpr bool FROM_LDS = false;
     uint4 k[G::KR][G::KC];
     uint32_t v[G::VR][G::VW];
 
@@ -269,55 +269,74 @@ struct Frag {
     }
 };
 
+// The query operand of 16 rows: fp32 pieces, or the 16-bit terms of each value,
+// in registers or in LDS.
+template <int TY, int D>
+struct QueryRegs {
+    uint4 v[TERMS<TY>][Tile<TY, D>::KC];
+    __device__ __forceinline__ uint4 get(int n, int c) const { return v[n][c]; }
+    __device__ __forceinline__ void put(int n, int c, const uint4 &x) { v[n][c] = x; }
+};
+template <int TY, int D>
+struct QueryLds {
+    static constexpr int BYTES = TERMS<TY> * Tile<TY, D>::KC * 1024;
+    char *p;            // the lane's 16 bytes of piece 0
+    int first, step;    // pieces that this wave puts there
+    __device__ __forceinline__ uint4 get(int n, int c) const {
+        return *(const uint4 *)(p + (n * Tile<TY, D>::KC + c) * 1024);
+    }
+    __device__ __forceinline__ void put(int n, int c, const uint4 &x) const {
+        if (c % step == first) *(uint4 *)(p + (n * Tile<TY, D>::KC + c) * 1024) = x;
+    }
+};
+
 // A wave's running state over its 16 rows.
 template <int TY, int D>
 struct Wave16 {
     using G = Tile<TY, D>;
-    static constexpr int NT = TERMS<TY>;
-    uint4 q[NT][G::KC];   // query operand: fp32 pieces, or the 16-bit terms of each value
     Score sc;
     float m, l;
     f32x4 o[G::DPL];   // o[t][r]: column DPL (4 (l / 16) + r) + t of row l % 16
 
-    __device__ __forceinline__ void init(const AttnArgs &a, const Row &r, int lane) {
-        const uint32_t g = lane >> 4;
-        const float *qp = a.q + ((uint64_t)(uint32_t)r.row * a.n_head + r.head) * D;
+    template <class Query>
+    __device__ __forceinline__ void init(const AttnArgs &a, const Row &r, int lane, Query &q) {
         constexpr int E = TY == ATTN_F32 ? 4 : 8;   // values per piece
+        const uint32_t g = lane >> 4;
+        const float *qp = a.q + ((uint64_t)(uint32_t)(r.valid ? r.row : 0) * a.n_head + r.head) * D + g * E;
         float v[G::KC][E];
         float top = 0.0f;
 #pragma unroll
         for (int c = 0; c < G::KC; c++)
 #pragma unroll
             for (int i = 0; i < E; i += 4) {
-                float4 x = make_float4(0, 0, 0, 0);
-                if (r.valid) x = *(const float4 *)(qp + c * (TY == ATTN_F32 ? 16 : 32) + g * E + i);
+                const float4 x = *(const float4 *)(qp + c * (TY == ATTN_F32 ? 16 : 32) + i);
                 v[c][i] = x.x, v[c][i + 1] = x.y, v[c][i + 2] = x.z, v[c][i + 3] = x.w;
-                top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
             }
-        float mul = a.scale;
-        if constexpr (TY == ATTN_F32) {
-#pragma unroll
-            for (int c = 0; c < G::KC; c++)
-                q[0][c] = make_uint4(__float_as_uint(v[c][0]), __float_as_uint(v[c][1]), __float_as_uint(v[c][2]),
-                                     __float_as_uint(v[c][3]));
-        } else {
+        float mul = a.scale, up = 1.0f;
+        if constexpr (TY == ATTN_F16) {
             // fp16 terms: the row is brought to 2^12 by a power of two, so
             // that neither a large q overflows nor a small one loses bits
-            float up = 1.0f;
-            if constexpr (TY == ATTN_F16) {
-                top = rows_max(top);
-                int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-                e = min(max(e, -100), 100);
-                up = __uint_as_float((uint32_t)(127 + 12 - e) << 23);
-                mul = a.scale * __uint_as_float((uint32_t)(127 - 12 + e) << 23);
-            }
 #pragma unroll
-            for (int c = 0; c < G::KC; c++) {
-                uint32_t w[4][NT];
+            for (int c = 0; c < G::KC; c++)
+#pragma unroll
+                for (int i = 0; i < E; i++) top = fmaxf(top, fabsf(v[c][i]));
+            top = rows_max(top);
+            int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+            e = min(max(e, -100), 100);
+            up = __uint_as_float((uint32_t)(127 + 12 - e) << 23);
+            mul = a.scale * __uint_as_float((uint32_t)(127 - 12 + e) << 23);
+        }
+#pragma unroll
+        for (int c = 0; c < G::KC; c++) {
+            if constexpr (TY == ATTN_F32) {
+                q.put(0, c, make_uint4(__float_as_uint(v[c][0]), __float_as_uint(v[c][1]), __float_as_uint(v[c][2]),
+                                       __float_as_uint(v[c][3])));
+            } else {
+                uint32_t w[4][TERMS<TY>];
 #pragma unroll
                 for (int i = 0; i < 4; i++) split<TY>(v[c][2 * i] * up, v[c][2 * i + 1] * up, w[i]);
 #pragma unroll
-                for (int n = 0; n < NT; n++) q[n][c] = make_uint4(w[0][n], w[1][n], w[2][n], w[3][n]);
+                for (int n = 0; n < TERMS<TY>; n++) q.put(n, c, make_uint4(w[0][n], w[1][n], w[2][n], w[3][n]));
             }
         }
         sc = make_score(a, r, mul);
@@ -379,47 +398,70 @@ struct Wave16 {
     }
 };
 
+// use(i, piece i) for i = 0 .. N-1, each piece asked for A uses ahead: an LDS
+// read takes about as long as two pieces' products. r: the pieces 0 .. A-1,
+// asked for before.
+template <int N, int A, class Load, class Use>
+__device__ __forceinline__ void ahead(uint4 (&r)[A + 1], Load load, Use use) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (i + A < N) r[(i + A) % (A + 1)] = load(i + A);
+        __builtin_amdgcn_sched_barrier(0);
+        use(i, r[i % (A + 1)]);
+    }
+}
+
 // One tile of keys for a wave's B blocks of 16 rows: every operand piece of K
 // and V is taken once for all of them.
-template <int TY, int D, int B, class Src>
-__device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Src &f, const Row (&row)[B], int32_t j0,
-                                          int32_t end, const bool (&whole)[B], int lane) {
+template <int TY, int D, int B, class Query, class Src>
+__device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Query (&q)[B], const Src &f, const Row (&row)[B],
+                                          int32_t j0, int32_t end, const bool (&whole)[B], int lane) {
     using G = Tile<TY, D>;
     constexpr int NT = TERMS<TY>;
+    constexpr int A = TY == ATTN_BF16 && D == 256 ? 1 : 2;   // 1: registers
     float y[B][G::VR];
+    f32x4 s[G::KR][B];
 #pragma unroll
-    for (int t = 0; t < G::KR; t++) {
-        f32x4 s[B];
+    for (int t = 0; t < G::KR; t++)
 #pragma unroll
-        for (int b = 0; b < B; b++) s[b] = f32x4{0, 0, 0, 0};
+        for (int b = 0; b < B; b++) s[t][b] = f32x4{0, 0, 0, 0};
+    auto product = [&](int i, const uint4 &k) {
+        const int c = i / G::KR, t = i % G::KR;   // neighbours add to different sums
 #pragma unroll
-        for (int c = 0; c < G::KC; c++) {
-            const uint4 k = f.key(t, c);
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int b = 0; b < B; b++) {
+                if constexpr (TY == ATTN_F32) {
+                    const f32x4 kv = bits<f32x4>(k), qv = bits<f32x4>(q[b].get(0, c));
 #pragma unroll
-                for (int b = 0; b < B; b++) {
-                    if constexpr (TY == ATTN_F32) {
-                        const f32x4 kv = bits<f32x4>(k), qv = bits<f32x4>(st[b].q[0][c]);
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[i], qv[i], s[b], 0, 0, 0);
-                    } else {
-                        s[b] = mfma32<TY>(k, st[b].q[n][c], s[b]);
-                    }
+                    for (int e = 0; e < 4; e++)
+                        s[t][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[e], qv[e], s[t][b], 0, 0, 0);
+                } else {
+                    s[t][b] = mfma32<TY>(k, q[b].get(n, c), s[t][b]);
                 }
-        }
+            }
+    };
+    constexpr int NK = G::KR * G::KC;
+    if constexpr (Src::FROM_LDS && TY != ATTN_F32) {
+        uint4 r[A + 1];
+#pragma unroll
+        for (int i = 0; i < A; i++) r[i] = f.key(i % G::KR, i / G::KR);
+        ahead<NK, A>(r, [&](int i) { return f.key(i % G::KR, i / G::KR); }, product);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NK; i++) product(i, f.key(i % G::KR, i / G::KR));
+    }
+#pragma unroll
+    for (int t = 0; t < G::KR; t++)
 #pragma unroll
         for (int b = 0; b < B; b++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[b][4 * t + r] = s[b][r];
-    }
+            for (int r = 0; r < 4; r++) y[b][4 * t + r] = s[t][b][r];
     // the first pieces of V are on their way while the weights are formed
-    constexpr int PRE = Src::PRE;
-    uint4 pre[PRE ? PRE : 1];
-    if constexpr (PRE) {
+    uint4 pre[A + 1];
+    if constexpr (Src::FROM_LDS && TY != ATTN_F32) {
 #pragma unroll
-        for (int t = 0; t < PRE; t++) pre[t] = f.value(t);
+        for (int i = 0; i < A; i++) pre[i] = f.value(i);
         asm volatile("" ::: "memory");
     }
 #pragma unroll
@@ -440,14 +482,18 @@ __device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Src &f, 
         for (int b = 0; b < B; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++) split<TY>(y[b][2 * i], y[b][2 * i + 1], pt[b][i]);
-#pragma unroll
-        for (int t = 0; t < G::DPL; t++) {
-            const uint4 vt = t < PRE ? pre[t < PRE ? t : 0] : f.value(t);
+        auto add = [&](int t, const uint4 &vt) {
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int b = 0; b < B; b++)
                     st[b].o[t] = mfma32<TY>(vt, make_uint4(pt[b][0][n], pt[b][1][n], pt[b][2][n], pt[b][3][n]), st[b].o[t]);
+        };
+        if constexpr (Src::FROM_LDS) {
+            ahead<G::DPL, A>(pre, [&](int t) { return f.value(t); }, add);
+        } else {
+#pragma unroll
+            for (int t = 0; t < G::DPL; t++) add(t, f.value(t));
         }
     }
 }
@@ -531,6 +577,7 @@ struct Item {
 };
 __device__ __forceinline__ Item make_item(const AttnArgs &a, uint32_t id) {
     Item it;
+    id += a.first_item;
     it.pooled = id >= a.own_items;
     if (it.pooled) id -= a.own_items;
     const uint32_t splits = it.pooled ? a.shared_splits : a.own_splits;
@@ -634,21 +681,22 @@ __device__ __forceinline__ void odd_rows(const AttnArgs &a, const Item &it, cons
 }
 
 // Few rows: the waves of a workgroup share 16 rows and take every W-th tile of
-// the keys, straight from memory into the operands' registers, the next tile's
-// on their way while one is worked on (where the registers hold two; with
-// 256-wide heads, and 128-wide ones of bf16 with their third terms, they do not,
-// and the waves cover for each other).
+// the keys, straight from memory into the operands' registers. Bound by
+// memory: what counts is how many loads are in flight, so the query operand,
+// the same for all waves, lies in LDS, and its registers hold more waves.
 constexpr int ROWS_WAVES = 4;
 template <int TY, int D, int W>
 struct RowsLds {
-    float o[W][16][D + 4];
+    union {
+        char q[QueryLds<TY, D>::BYTES];
+        float o[W][16][D + 4];
+    };
     float m[W][16], l[W][16];
     uint64_t at[16];   // packed row x head of each row, ~0 for none
 };
 template <int TY, int D, int W>
 __device__ __forceinline__ void attn_rows_item(const AttnArgs &a, const Item &it, char *shared) {
     using G = Tile<TY, D>;
-    constexpr bool AHEAD = D == 64 || (D == 128 && TY != ATTN_BF16);
     auto &lds = *(RowsLds<TY, D, W> *)shared;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     SeqRows sr;
@@ -659,7 +707,8 @@ __device__ __forceinline__ void attn_rows_item(const AttnArgs &a, const Item &it
     int32_t c0, c1;
     split_share(a, it, sp.lo, sp.hi, G::KT, c0, c1);
 
-    // the wave's first tile is asked for before q is waited for
+    // the wave's first tile is asked for before q is waited for (with 256-wide
+    // heads there are no registers for both)
     Segment g = segment(a, G::EB, it.kvh, it.seq, true, c0, c1);
     int32_t j = g.c0 + wave * G::KT;
     bool own = false;
@@ -669,34 +718,26 @@ __device__ __forceinline__ void attn_rows_item(const AttnArgs &a, const Item &it
         own = true;
     }
     Frag<TY, D> f;
-    bool some = j < g.c1;
-    if (some) f.load(g.k, g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
+    if (D <= 128 && j < g.c1) f.load(g.k, g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
     Wave16<TY, D> sts[1], &st = sts[0];
-    st.init(a, row, lane);
-    while (some) {
-        Segment gn = g;
-        int32_t jn = j + W * G::KT;
-        if (jn >= g.c1 && !own) {
-            gn = segment(a, G::EB, it.kvh, it.seq, false, c0, c1);
-            jn = gn.c0 + wave * G::KT;
+    QueryLds<TY, D> q[1] = {{lds.q + lane * 16, wave, W}};
+    st.init(a, row, lane, q[0]);
+    __syncthreads();
+    if (D > 128 && j < g.c1) f.load(g.k, g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
+    while (j < g.c1) {
+        const bool whole[1] = {j >= sp.all_lo && j + G::KT <= min(sp.all_hi, g.c1)};
+        asm volatile("" ::: "memory");   // q's pieces are read again for each tile, not kept
+        attn_step<TY, D, 1>(sts, q, f, rows, j, g.c1, whole, lane);
+        j += W * G::KT;
+        if (j >= g.c1 && !own) {
+            g = segment(a, G::EB, it.kvh, it.seq, false, c0, c1);
+            j = g.c0 + wave * G::KT;
             own = true;
         }
-        const bool more = jn < gn.c1;
-        const bool whole[1] = {j >= sp.all_lo && j + G::KT <= min(sp.all_hi, g.c1)};
-        if constexpr (AHEAD) {
-            Frag<TY, D> fn;
-            if (more) fn.load(gn.k, gn.v, gn.row_bytes, jn - gn.origin, gn.c1 - gn.origin, lane);
-            attn_step<TY, D, 1>(sts, f, rows, j, g.c1, whole, lane);
-            f = fn;
-        } else {
-            attn_step<TY, D, 1>(sts, f, rows, j, g.c1, whole, lane);
-            if (more) f.load(gn.k, gn.v, gn.row_bytes, jn - gn.origin, gn.c1 - gn.origin, lane);
-        }
-        g = gn;
-        j = jn;
-        some = more;
+        if (j < g.c1) f.load(g.k, g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
     }
     st.l = rows_sum(st.l);
+    __syncthreads();   // q is done with: its LDS takes the sums
     odd_rows<TY, D, W>(a, it, row, c0, c1, wave, lane, st, &lds.o[wave][0][0]);
 
     // the waves' sums of the same rows, joined in LDS
@@ -761,23 +802,25 @@ __device__ __forceinline__ void attn_rows_item(const AttnArgs &a, const Item &it
 template <int TY, int D, int NTHREADS>
 struct Stage {
     using G = Tile<TY, D>;
-    static constexpr int NK = TY == ATTN_F32 || (TY == ATTN_BF16 && D == 256) || (TY == ATTN_F16 && D == 128) ? 32 : 64;   // 32: registers
+    static constexpr int NK = D * G::EB > 256 ? 32 * (NTHREADS / 256) : 64;
     static constexpr int KROW = D * G::EB + 16, VBYTES = TY == ATTN_F32 ? NK * KROW : NK * D * 2;
     static constexpr int BYTES = NK * KROW + VBYTES;
     static constexpr int PER_ROW = D * G::EB / 16;                            // 16-byte pieces of a row
-    static constexpr int KN = NK * PER_ROW / NTHREADS;                        // pieces of K per thread
-    static constexpr int UNITS = NK / 4 * (D / 4);                            // 4 x 4 blocks of V
+    static constexpr int FK = 32;                                             // keys of a part
+    static constexpr int PARTS = NK / FK;
+    static constexpr int KN = FK * PER_ROW / NTHREADS;                        // pieces of K per thread
+    static constexpr int UNITS = FK / 4 * (D / 4);                            // 4 x 4 blocks of V
     static constexpr int VN = (UNITS + NTHREADS - 1) / NTHREADS;              // blocks per thread
-    static_assert(NK * PER_ROW % NTHREADS == 0, "whole pieces per thread");
+    static_assert(FK * PER_ROW % NTHREADS == 0, "whole pieces per thread");
 
     u32x4 k[KN];
     uint2 v[TY == ATTN_F32 ? 2 * KN : VN * 4];
 
-    // rows j0 .. j0 + NK from memory; rows from `end` on repeat the last one before it
+    // rows j0 .. j0 + FK from memory; rows from `end` on repeat the last one before it
     __device__ __forceinline__ void fetch(const char *kb, const char *vb, uint32_t row_bytes, int32_t j0, int32_t end) {
         const uint64_t at = (uint64_t)(uint32_t)j0 * row_bytes;
         const char *kp = kb + at, *vp = vb + at;
-        const uint32_t last = (uint32_t)min(end - j0, NK) - 1;
+        const uint32_t last = (uint32_t)min(end - j0, FK) - 1;
 #pragma unroll
         for (int n = 0; n < KN; n++) {
             const uint32_t id = threadIdx.x + NTHREADS * n;
@@ -800,13 +843,15 @@ struct Stage {
             }
         }
     }
-    __device__ __forceinline__ void store(char *lds) const {
+    // into part `part` of a stage
+    __device__ __forceinline__ void store(char *lds, int part) const {
+        char *kl = lds + part * FK * KROW, *vl = lds + NK * KROW + part * (TY == ATTN_F32 ? FK * KROW : FK * D * 2);
 #pragma unroll
         for (int n = 0; n < KN; n++) {
             const uint32_t id = threadIdx.x + NTHREADS * n;
-            *(u32x4 *)(lds + id / PER_ROW * KROW + id % PER_ROW * 16) = k[n];
+            *(u32x4 *)(kl + id / PER_ROW * KROW + id % PER_ROW * 16) = k[n];
             if constexpr (TY == ATTN_F32)
-                *(uint4 *)(lds + NK * KROW + id / PER_ROW * KROW + id % PER_ROW * 16) =
+                *(uint4 *)(vl + id / PER_ROW * KROW + id % PER_ROW * 16) =
                     make_uint4(v[2 * n].x, v[2 * n].y, v[2 * n + 1].x, v[2 * n + 1].y);
         }
         if constexpr (TY != ATTN_F32) {
@@ -814,10 +859,10 @@ struct Stage {
             for (int n = 0; n < VN; n++) {
                 const uint32_t id = threadIdx.x + NTHREADS * n;
                 if (UNITS % NTHREADS == 0 || id < UNITS) {
-                    // rows 4 q .. of subtile q / 8: half (q / 4) % 2 of the operand's keys, lane row q % 4
+                    // rows 4 q ..: half q / 4 of the operand's keys, lane row q % 4
                     const uint32_t q = id / (D / 4), col = id % (D / 4) * 4;
-                    const uint32_t sub = q / 8, half = q / 4 % 2, lane0 = q % 4 * 16 + col / G::DPL, t0 = col % G::DPL;
-                    char *p = lds + NK * KROW + sub * (32 * D * 2) + (t0 * 64 + lane0) * 16 + half * 8;
+                    const uint32_t half = q / 4, lane0 = q % 4 * 16 + col / G::DPL, t0 = col % G::DPL;
+                    char *p = vl + (t0 * 64 + lane0) * 16 + half * 8;
                     const uint2 *x = v + 4 * n;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
@@ -833,7 +878,7 @@ struct Stage {
     }
     // the operands of one of its tiles, as Frag gives them
     struct View {
-        static constexpr int PRE = TY == ATTN_F32 || D == 256 ? 0 : 4;
+        static constexpr bool FROM_LDS = true;
         const char *kp, *vp;
         __device__ __forceinline__ uint4 key(int t, int i) const { return *(const uint4 *)(kp + t * 16 * KROW + i * 64); }
         __device__ __forceinline__ uint4 value(int t) const { return *(const uint4 *)(vp + t * 1024); }
@@ -892,30 +937,39 @@ __device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it
     split_share(a, it, lo, hi, S::NK, c0, c1);
 
     Wave16<TY, D> st[B];
+    QueryRegs<TY, D> q[B];
 #pragma unroll
-    for (int b = 0; b < B; b++) st[b].init(a, row[b], lane);
+    for (int b = 0; b < B; b++) st[b].init(a, row[b], lane, q[b]);
     S stage;
     for (int sg = 0; sg < 2; sg++) {
         const Segment g = segment(a, G::EB, it.kvh, it.seq, sg == 0, c0, c1);
         if (g.c0 >= g.c1) continue;
-        stage.fetch(g.k, g.v, g.row_bytes, g.c0 - g.origin, g.c1 - g.origin);
         int at = 0;
         __syncthreads();   // the last segment's readers are done
-        stage.store(lds.stage[0]);
+#pragma unroll 1
+        for (int part = 0; part < S::PARTS; part++) {
+            if (g.c0 + part * S::FK >= g.c1) break;
+            stage.fetch(g.k, g.v, g.row_bytes, g.c0 + part * S::FK - g.origin, g.c1 - g.origin);
+            stage.store(lds.stage[0], part);
+        }
         __syncthreads();
         for (int32_t j = g.c0; j < g.c1; j += S::NK) {
-            const bool more = j + S::NK < g.c1;
-            if (more) stage.fetch(g.k, g.v, g.row_bytes, j + S::NK - g.origin, g.c1 - g.origin);
 #pragma unroll 1
-            for (int sub = 0; sub < S::NK / G::KT; sub++) {
-                const int32_t js = j + sub * G::KT;
-                if (js >= min(wave_hi, g.c1) || js + G::KT <= wave_lo) continue;
-                bool whole[B];
+            for (int part = 0; part < S::PARTS; part++) {
+                // the same part of the next stage is on its way while this one is worked on
+                const int32_t jn = j + S::NK + part * S::FK;
+                if (jn < g.c1) stage.fetch(g.k, g.v, g.row_bytes, jn - g.origin, g.c1 - g.origin);
+#pragma unroll 1
+                for (int sub = part * (S::FK / G::KT); sub < (part + 1) * (S::FK / G::KT); sub++) {
+                    const int32_t js = j + sub * G::KT;
+                    if (js >= min(wave_hi, g.c1) || js + G::KT <= wave_lo) continue;
+                    bool whole[B];
 #pragma unroll
-                for (int b = 0; b < B; b++) whole[b] = js >= sp[b].all_lo && js + G::KT <= min(sp[b].all_hi, g.c1);
-                attn_step<TY, D, B>(st, S::view(lds.stage[at], sub, lane), row, js, g.c1, whole, lane);
+                    for (int b = 0; b < B; b++) whole[b] = js >= sp[b].all_lo && js + G::KT <= min(sp[b].all_hi, g.c1);
+                    attn_step<TY, D, B>(st, q, S::view(lds.stage[at], sub, lane), row, js, g.c1, whole, lane);
+                }
+                if (jn < g.c1) stage.store(lds.stage[at ^ 1], part);
             }
-            if (more) stage.store(lds.stage[at ^ 1]);
             __syncthreads();
             at ^= 1;
         }
@@ -949,7 +1003,7 @@ __device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it
 // together (many rows) beside each sequence's own keys (few rows), in one
 // launch, so that matrix work and memory traffic overlap.
 template <int TY, int D>
-__global__ void __launch_bounds__(64 * ROWS_WAVES, D == 256 ? 1 : 2) k_attn(const AttnArgs a) {
+__global__ void __launch_bounds__(64 * ROWS_WAVES, D == 64 ? 4 : D == 128 ? (TY == ATTN_F32 ? 3 : 2) : TY == ATTN_F32 ? 2 : 1) k_attn(const AttnArgs a) {
     __shared__ __align__(16) char lds[sizeof(RowsLds<TY, D, ROWS_WAVES>)];
     attn_rows_item<TY, D, ROWS_WAVES>(a, make_item(a, blockIdx.x), lds);
 }
@@ -963,7 +1017,7 @@ __global__ void __launch_bounds__((64 * TILE_WAVES<TY, D>), 2) k_attn_tile(const
     attn_tile_item<TY, D, B, W>(a, make_item(a, blockIdx.x), lds);
 }
 template <int TY, int D>
-__global__ void __launch_bounds__(64 * ROWS_WAVES, D == 256 ? 1 : 2) k_attn_mixed(const AttnArgs a) {
+__global__ void __launch_bounds__(64 * ROWS_WAVES, 2) k_attn_mixed(const AttnArgs a) {
     constexpr int W = ROWS_WAVES;
     constexpr size_t R = sizeof(RowsLds<TY, D, W>), T = sizeof(TileLds<TY, D, 1, W>);
     __shared__ __align__(16) char lds[R > T ? R : T];
@@ -1027,17 +1081,29 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
 }
 
 template <int TY, int D>
-static hipError_t attn_run(const AttnArgs &a, AttnForm form, uint32_t items, hipStream_t s) {
-    const dim3 g(items);
-    if (form == ATTN_TILES) hipLaunchKernelGGL((k_attn_tile<TY, D>), g, dim3(64 * TILE_WAVES<TY, D>), 0, s, a);
-    else if (form == ATTN_MIXED) hipLaunchKernelGGL((k_attn_mixed<TY, D>), g, dim3(64 * ROWS_WAVES), 0, s, a);
-    else hipLaunchKernelGGL((k_attn<TY, D>), g, dim3(64 * ROWS_WAVES), 0, s, a);
+static hipError_t attn_run(AttnArgs a, const AttnPlan &p, hipStream_t s) {
+    const dim3 rows(64 * ROWS_WAVES), tile(64 * TILE_WAVES<TY, D>);
+    a.first_item = 0;
+    if (p.form == ATTN_TILES) {
+        hipLaunchKernelGGL((k_attn_tile<TY, D>), dim3(p.own_items), tile, 0, s, a);
+    } else if (p.form == ATTN_ROWS) {
+        hipLaunchKernelGGL((k_attn<TY, D>), dim3(p.own_items + p.shared_items), rows, 0, s, a);
+    } else if constexpr (D <= 128) {
+        hipLaunchKernelGGL((k_attn_mixed<TY, D>), dim3(p.own_items + p.shared_items), rows, 0, s, a);
+    } else {
+        // no registers for both in one kernel
+        hipLaunchKernelGGL((k_attn<TY, D>), dim3(p.own_items), rows, 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        a.first_item = p.own_items;
+        hipLaunchKernelGGL((k_attn_tile<TY, D>), dim3(p.shared_items), tile, 0, s, a);
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !a.slots) return e;
-    // four waves a row where many slots meet and there are few rows
-    const uint32_t rows = a.n_seq * a.max_q;
-    if (a.slots > 8) hipLaunchKernelGGL((k_attn_join<D, 4>), dim3(rows * a.n_head), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_attn_join<D, 1>), dim3(rows * ((a.n_head + 3) / 4)), dim3(256), 0, s, a);
+    // four waves a row where many slots meet
+    const uint32_t n = a.n_seq * a.max_q;
+    if (a.slots > 8) hipLaunchKernelGGL((k_attn_join<D, 4>), dim3(n * a.n_head), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_join<D, 1>), dim3(n * ((a.n_head + 3) / 4)), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
@@ -1052,12 +1118,11 @@ hipError_t launch_attn(AttnArgs a, uint32_t type, uint32_t head_dim, const AttnP
     a.shared_chunk = p.shared_chunk;
     a.acc = (float *)scratch;
     a.ml = (float2 *)((char *)scratch + (uint64_t)a.n_rows * a.n_head * p.slots * head_dim * 4);
-    const uint32_t items = p.own_items + p.shared_items;
     auto go = [&](auto ty) -> hipError_t {
         constexpr int TY = decltype(ty)::value;
-        if (head_dim == 64) return attn_run<TY, 64>(a, p.form, items, s);
-        if (head_dim == 128) return attn_run<TY, 128>(a, p.form, items, s);
-        return attn_run<TY, 256>(a, p.form, items, s);
+        if (head_dim == 64) return attn_run<TY, 64>(a, p, s);
+        if (head_dim == 128) return attn_run<TY, 128>(a, p, s);
+        return attn_run<TY, 256>(a, p, s);
     };
     if (type == ATTN_F32) return go(std::integral_constant<int, ATTN_F32>());
     if (type == ATTN_F16) return go(std::integral_constant<int, ATTN_F16>());

@@ -128,7 +128,9 @@ inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint3
     if (n_shared && n_seq > 1 && !tiles && cap >= 2) {
         const uint64_t pooled = (uint64_t)n_rows * group;
         p.form = pooled > ATTN_FEW_ROWS ? ATTN_MIXED : ATTN_ROWS;
-        p.shared_tiles = (uint32_t)cover(pooled, p.form == ATTN_MIXED ? 16 * waves : 16);
+        // (a mixed launch's tiles are of 16 rows a wave; 256-wide heads take two launches)
+        const uint32_t wide = head_dim == 256 ? (uint32_t)attn_tile_rows(type, 256) : 16 * waves;
+        p.shared_tiles = (uint32_t)cover(pooled, p.form == ATTN_MIXED ? wide : 16);
         split((uint64_t)n_kv * p.shared_tiles, n_shared, 2 * cus, p.form == ATTN_MIXED ? many : few, cap / 2,
               p.shared_splits, p.shared_chunk);
         split(own, max_kv, 2 * cus, few, cap - p.shared_splits, p.own_splits, p.own_chunk);

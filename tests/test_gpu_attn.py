@@ -176,6 +176,18 @@ def test_shared(hip, t, D, n_seq, rows, own, shared):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("how", ["bare", "cap", "bias"])
+@pytest.mark.parametrize("n_seq,rows,shared", [(3, 1, 32), (9, 3, 32), (9, 3, 33), (20, 1, 700), (40, 2, 64), (2, 8, 300)])
+def test_shared_few_and_many_rows(hip, t, D, how, n_seq, rows, shared):
+    """Rows of all sequences together from a few (12) to several tiles, one
+    stage of shared keys and many."""
+    rng = np.random.default_rng(n_seq + shared)
+    check(hip, O.make(rng, n_seq, [rows] * n_seq, [20] * n_seq, 20, 8, 2, D, t, n_shared=shared, alibi=how == "bias",
+                      softcap=20.0 if how == "cap" else 0.0))
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
 def test_shared_masks(hip, t):
     """Documents and prefixes that end inside the shared keys, sequences
     without rows or own keys, a cap."""
