@@ -212,6 +212,7 @@ template <int TY, int D>
 struct Frag {
     using G = Tile<TY, D>;
     static constexpr bool FROM_LDS = false;
+    static constexpr int KR = G::KR;
     uint4 k[G::KR][G::KC];
     uint32_t v[G::VR][G::VW];
 
@@ -348,7 +349,8 @@ struct Wave16 {
 
     // The weights of one tile from its products, and the running maximum and sum; keys
     // from `end` on are not of its segment; whole: the row sees all of them.
-    __device__ __forceinline__ void weights(float (&y)[G::VR], const Row &row, int32_t j0, int32_t end, bool whole,
+    template <int VR>
+    __device__ __forceinline__ void weights(float (&y)[VR], const Row &row, int32_t j0, int32_t end, bool whole,
                                             int lane) {
         const int32_t g4 = 4 * (lane >> 4);
         // with neither cap nor bias the product's factor goes into the exponent's
@@ -359,14 +361,14 @@ struct Wave16 {
         if (!whole) {
             const int32_t hi = min(row.hi, end);
 #pragma unroll
-            for (int r = 0; r < G::VR; r++) {
+            for (int r = 0; r < VR; r++) {
                 const int32_t j = j0 + (r >> 2) * 16 + g4 + (r & 3);
                 if (j < row.lo || j >= hi) y[r] = NEG_INF;
             }
         }
         float top = y[0];
 #pragma unroll
-        for (int r = 1; r < G::VR; r++) top = fmaxf(top, y[r]);
+        for (int r = 1; r < VR; r++) top = fmaxf(top, y[r]);
         top = rows_max(top) * mul;
         // the maximum that scales the sums moves only when it falls behind by
         // 2^8: most tiles then leave the accumulators alone
@@ -381,7 +383,7 @@ struct Wave16 {
         // fp16 terms of p stand 2^7 higher, so that the second ones stay normal
         const float base = (m == NEG_INF ? 0.0f : m) - (TY == ATTN_F16 ? 7.0f : 0.0f);
 #pragma unroll
-        for (int r = 0; r < G::VR; r++) {
+        for (int r = 0; r < VR; r++) {
             y[r] = exp2_hw(fmaf(y[r], mul, -base));
             l += y[r];
         }
@@ -417,16 +419,16 @@ template <int TY, int D, int B, class Query, class Src>
 __device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Query (&q)[B], const Src &f, const Row (&row)[B],
                                           int32_t j0, int32_t end, const bool (&whole)[B], int lane) {
     using G = Tile<TY, D>;
-    constexpr int NT = TERMS<TY>;
+    constexpr int NT = TERMS<TY>, KR = Src::KR, VR = 4 * KR;
     constexpr int A = TY == ATTN_BF16 && D == 256 ? 1 : 2;   // 1: registers
-    float y[B][G::VR];
-    f32x4 s[G::KR][B];
+    float y[B][VR];
+    f32x4 s[KR][B];
 #pragma unroll
-    for (int t = 0; t < G::KR; t++)
+    for (int t = 0; t < KR; t++)
 #pragma unroll
         for (int b = 0; b < B; b++) s[t][b] = f32x4{0, 0, 0, 0};
     auto product = [&](int i, const uint4 &k) {
-        const int c = i / G::KR, t = i % G::KR;   // neighbours add to different sums
+        const int c = i / KR, t = i % KR;   // neighbours add to different sums
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -441,18 +443,18 @@ __device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Query (&
                 }
             }
     };
-    constexpr int NK = G::KR * G::KC;
+    constexpr int NK = KR * G::KC;
     if constexpr (Src::FROM_LDS && TY != ATTN_F32) {
         uint4 r[A + 1];
 #pragma unroll
-        for (int i = 0; i < A; i++) r[i] = f.key(i % G::KR, i / G::KR);
-        ahead<NK, A>(r, [&](int i) { return f.key(i % G::KR, i / G::KR); }, product);
+        for (int i = 0; i < A; i++) r[i] = f.key(i % KR, i / KR);
+        ahead<NK, A>(r, [&](int i) { return f.key(i % KR, i / KR); }, product);
     } else {
 #pragma unroll
-        for (int i = 0; i < NK; i++) product(i, f.key(i % G::KR, i / G::KR));
+        for (int i = 0; i < NK; i++) product(i, f.key(i % KR, i / KR));
     }
 #pragma unroll
-    for (int t = 0; t < G::KR; t++)
+    for (int t = 0; t < KR; t++)
 #pragma unroll
         for (int b = 0; b < B; b++)
 #pragma unroll
@@ -468,7 +470,7 @@ __device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Query (&
     for (int b = 0; b < B; b++) st[b].weights(y[b], row[b], j0, end, whole[b], lane);
     if constexpr (TY == ATTN_F32) {
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+        for (int r = 0; r < VR; r++)
 #pragma unroll
             for (int t = 0; t < G::DPL; t++) {
                 const float v = f.value(r, t);
@@ -802,12 +804,14 @@ __device__ __forceinline__ void attn_rows_item(const AttnArgs &a, const Item &it
 template <int TY, int D, int NTHREADS>
 struct Stage {
     using G = Tile<TY, D>;
-    static constexpr int NK = D * G::EB > 256 ? 32 * (NTHREADS / 256) : 64;
+    // keys of a stage: few enough for two workgroups on a CU (fp32, 64 wide: four)
+    static constexpr int NK = TY == ATTN_F32 ? (D == 256 ? 16 : 32) : D == 256 ? 32 * (NTHREADS / 256) : 64;
     static constexpr int KROW = D * G::EB + 16, VBYTES = TY == ATTN_F32 ? NK * KROW : NK * D * 2;
     static constexpr int BYTES = NK * KROW + VBYTES;
     static constexpr int PER_ROW = D * G::EB / 16;                            // 16-byte pieces of a row
-    static constexpr int FK = 32;                                             // keys of a part
+    static constexpr int FK = NK < 32 ? NK : 32;                              // keys of a part
     static constexpr int PARTS = NK / FK;
+    static constexpr int SK = FK;                                             // keys worked on at a time
     static constexpr int KN = FK * PER_ROW / NTHREADS;                        // pieces of K per thread
     static constexpr int UNITS = FK / 4 * (D / 4);                            // 4 x 4 blocks of V
     static constexpr int VN = (UNITS + NTHREADS - 1) / NTHREADS;              // blocks per thread
@@ -879,16 +883,17 @@ struct Stage {
     // the operands of one of its tiles, as Frag gives them
     struct View {
         static constexpr bool FROM_LDS = true;
+        static constexpr int KR = SK / 16;
         const char *kp, *vp;
         __device__ __forceinline__ uint4 key(int t, int i) const { return *(const uint4 *)(kp + t * 16 * KROW + i * 64); }
         __device__ __forceinline__ uint4 value(int t) const { return *(const uint4 *)(vp + t * 1024); }
-        __device__ __forceinline__ float value(int r, int t) const { return *(const float *)(vp + r * KROW + t * 4); }
+        __device__ __forceinline__ float value(int r, int t) const { return *(const float *)(vp + ((r >> 2) * 16 + (r & 3)) * KROW + t * 4); }
     };
     static __device__ __forceinline__ View view(const char *lds, int sub, int lane) {
         View w;
         const int c = lane & 15, g = lane >> 4;
-        w.kp = lds + (sub * G::KT + c) * KROW + g * 16;
-        if constexpr (TY == ATTN_F32) w.vp = lds + NK * KROW + (sub * G::KT + 4 * g) * KROW + c * (G::DPL * 4);
+        w.kp = lds + (sub * SK + c) * KROW + g * 16;
+        if constexpr (TY == ATTN_F32) w.vp = lds + NK * KROW + (sub * SK + 4 * g) * KROW + c * (G::DPL * 4);
         else w.vp = lds + NK * KROW + sub * (32 * D * 2) + lane * 16;
         return w;
     }
@@ -959,14 +964,12 @@ __device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it
                 // the same part of the next stage is on its way while this one is worked on
                 const int32_t jn = j + S::NK + part * S::FK;
                 if (jn < g.c1) stage.fetch(g.k, g.v, g.row_bytes, jn - g.origin, g.c1 - g.origin);
-#pragma unroll 1
-                for (int sub = part * (S::FK / G::KT); sub < (part + 1) * (S::FK / G::KT); sub++) {
-                    const int32_t js = j + sub * G::KT;
-                    if (js >= min(wave_hi, g.c1) || js + G::KT <= wave_lo) continue;
+                const int32_t js = j + part * S::SK;
+                if (js < min(wave_hi, g.c1) && js + S::SK > wave_lo) {
                     bool whole[B];
 #pragma unroll
-                    for (int b = 0; b < B; b++) whole[b] = js >= sp[b].all_lo && js + G::KT <= min(sp[b].all_hi, g.c1);
-                    attn_step<TY, D, B>(st, q, S::view(lds.stage[at], sub, lane), row, js, g.c1, whole, lane);
+                    for (int b = 0; b < B; b++) whole[b] = js >= sp[b].all_lo && js + S::SK <= min(sp[b].all_hi, g.c1);
+                    attn_step<TY, D, B>(st, q, S::view(lds.stage[at], part, lane), row, js, g.c1, whole, lane);
                 }
                 if (jn < g.c1) stage.store(lds.stage[at ^ 1], part);
             }
