@@ -62,14 +62,17 @@ __device__ __forceinline__ float rows_sum(float v) {
 // tanh to about 1e-7 of its value: below 1 the continued fraction
 // u / (1 + u^2 / (3 + u^2 / (5 + u^2 / (7 + u^2 / 9)))), above it
 // 1 - 2 / (e^2u + 1), both over one reciprocal. NaN stays NaN.
+__device__ __forceinline__ float tanh_num(float u, float u2) { return u * fmaf(u2, u2 + 105.0f, 945.0f); }
+__device__ __forceinline__ float tanh_den(float u2) { return fmaf(u2, fmaf(u2, 15.0f, 420.0f), 945.0f); }
+__device__ __forceinline__ float tanh_below_1(float u) {
+    const float u2 = u * u;
+    return tanh_num(u, u2) * __builtin_amdgcn_rcpf(tanh_den(u2));
+}
 __device__ __forceinline__ float tanh_fast(float u) {
     const float u2 = u * u;
     const bool small = fabsf(u) < 1.0f;
-    const float num = u * fmaf(u2, u2 + 105.0f, 945.0f);
-    const float t = exp2_hw(u * (2.0f * LOG2E));
-    const float den = small ? fmaf(u2, fmaf(u2, 15.0f, 420.0f), 945.0f) : t + 1.0f;
-    const float r = __builtin_amdgcn_rcpf(den);
-    return small ? num * r : fmaf(-2.0f, r, 1.0f);
+    const float r = __builtin_amdgcn_rcpf(small ? tanh_den(u2) : exp2_hw(u * (2.0f * LOG2E)) + 1.0f);
+    return small ? tanh_num(u, u2) * r : fmaf(-2.0f, r, 1.0f);
 }
 
 // Two fp32 values as 16-bit terms each, every term packed: the first takes the
@@ -125,8 +128,23 @@ __device__ __forceinline__ Score make_score(const AttnArgs &a, const Row &r, flo
 template <int N, class Off>
 __device__ __forceinline__ void scores(const Score &c, float (&y)[N], int32_t pos0, Off off) {
     if (c.capped) {
+        // scores well below the cap, as almost all are, need no exponential
+        float most = 0.0f;
 #pragma unroll
-        for (int r = 0; r < N; r++) y[r] = c.cap * tanh_fast(y[r] * c.mul);
+        for (int r = 0; r < N; r++) {
+            y[r] *= c.mul;
+            most = fmaxf(most, fabsf(y[r]));
+        }
+        if (__any(most >= 1.0f)) {   // (NaN passes through either way)
+#pragma unroll
+            for (int r = 0; r < N; r++) {
+                y[r] = c.cap * tanh_fast(y[r]);
+                __builtin_amdgcn_sched_barrier(0);   // one after another: the rare way takes no registers of the other
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < N; r++) y[r] = c.cap * tanh_below_1(y[r]);
+        }
     } else {
 #pragma unroll
         for (int r = 0; r < N; r++) y[r] *= c.mul;
@@ -946,6 +964,7 @@ __device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it
 #pragma unroll
     for (int b = 0; b < B; b++) st[b].init(a, row[b], lane, q[b]);
     S stage;
+    if (W == 8 ? wave >= 4 : (blockIdx.x >> 8) & 1) __builtin_amdgcn_s_setprio(1);
     for (int sg = 0; sg < 2; sg++) {
         const Segment g = segment(a, G::EB, it.kvh, it.seq, sg == 0, c0, c1);
         if (g.c0 >= g.c1) continue;
@@ -980,6 +999,11 @@ __device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it
 #pragma unroll
     for (int b = 0; b < B; b++) {
         st[b].l = rows_sum(st[b].l);
+        // which row and head it was is worked out again: two registers less in the loop
+        uint32_t packed = it.tile * ROWS + (wave * B + b) * 16 + (lane & 15);
+        asm volatile("" : "+v"(packed));
+        row[b].row = sr.first + (int32_t)(packed / a.group);
+        row[b].head = it.kvh * a.group + packed % a.group;
         odd_rows<TY, D, 1>(a, it, row[b], c0, c1, 0, lane, st[b], (float *)lds.stage[0] + wave * D);
         if (!row[b].valid) continue;
         float *dst;
@@ -1006,7 +1030,7 @@ __device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it
 // together (many rows) beside each sequence's own keys (few rows), in one
 // launch, so that matrix work and memory traffic overlap.
 template <int TY, int D>
-__global__ void __launch_bounds__(64 * ROWS_WAVES, D == 64 ? 4 : D == 128 ? (TY == ATTN_F32 ? 3 : 2) : TY == ATTN_F32 ? 2 : 1) k_attn(const AttnArgs a) {
+__global__ void __launch_bounds__(64 * ROWS_WAVES, D == 64 ? (TY == ATTN_BF16 ? 3 : 4) : D == 128 ? (TY == ATTN_F32 ? 3 : 2) : TY == ATTN_F32 ? 2 : 1) k_attn(const AttnArgs a) {
     __shared__ __align__(16) char lds[sizeof(RowsLds<TY, D, ROWS_WAVES>)];
     attn_rows_item<TY, D, ROWS_WAVES>(a, make_item(a, blockIdx.x), lds);
 }
