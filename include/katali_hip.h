@@ -186,10 +186,12 @@ int katali_hip_rmsnorm_matvec_f32(const float *x_dev, const float *delta_dev, fl
  * products keep 22 bits of q and of the weights (fp16 caches) or all 24.
  *
  * Limits: head_dim 64, 128 or 256; n_head a multiple of n_kv_head, <= 1024;
- * n_seq <= 65535; q, k, v, out 16-byte aligned, cache strides multiples of 16
- * bytes, a row stride under 2^27 bytes; q and out do not overlap. Sums of split rows go through a library
- * scratch (64 MB, allocated by the first call, which must be outside graph
- * capture); calls that overlap on one GPU share it and race. */
+ * n_seq <= 65535; n_rows <= 2^22; n_rows * n_head and n_seq * max_q * n_head
+ * under 2^24; q, k, v, out 16-byte aligned, cache strides multiples of 16
+ * bytes, a row stride under 2^27 bytes; q and out do not overlap. Sums of
+ * split rows go through a library scratch (64 MB, allocated by the first
+ * call, which must be outside graph capture); calls that overlap on one GPU
+ * share it and race. */
 typedef struct KataliHipAttn {
     uint32_t struct_size;                  /* sizeof(KataliHipAttn) */
     uint32_t kv_type;                      /* F32, F16 or BF16: the caches' values */

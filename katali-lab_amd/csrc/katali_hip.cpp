@@ -449,10 +449,13 @@ int attn_shape(const KataliHipAttn *a, const KataliHipAttnPrefix *p) {
         return fail(KATALI_HIP_E_INVALID, "n_rows=%u max_q=%u without q_start (one row per sequence: %u and 1)", a->n_rows,
                     a->max_q, a->n_seq);
     if (!a->kv_len) return fail(KATALI_HIP_E_INVALID, "null kv_len");
-    // row counts that the kernels' 32-bit grids and row indexes hold
+    // a launch holds fewer than 2^32 threads: 256 for each (sequence, row, head), 512 for
+    // the heads of a row in kv_append
     const uint64_t per_seq = a->max_q < a->n_rows ? a->max_q : a->n_rows;
-    if ((uint64_t)a->n_rows * a->n_head > 0x7FFF0000ull || (uint64_t)a->n_seq * per_seq * a->n_head > 0x7FFF0000ull)
-        return fail(KATALI_HIP_E_UNSUPPORTED, "n_rows=%u n_seq=%u max_q=%u n_head=%u: above 2^31 rows x heads", a->n_rows,
+    if (a->n_rows > (1u << 22) || (uint64_t)a->n_rows * a->n_head >= (1u << 24) ||
+        (uint64_t)a->n_seq * per_seq * a->n_head >= (1u << 24))
+        return fail(KATALI_HIP_E_UNSUPPORTED,
+                    "n_rows=%u n_seq=%u max_q=%u n_head=%u: above 2^22 rows or 2^24 sequences x rows x heads", a->n_rows,
                     a->n_seq, a->max_q, a->n_head);
     const uint64_t n_prefix = p ? p->n_prefix : 0;
     if (n_prefix + a->max_kv >= 0x7FFFF000ull)

@@ -11,9 +11,16 @@
  *                                    at the engine's shapes (criteria printed)
  *   katali-hip check-moe             the fused MoE layer against the CPU's q8_1
  *                                    path (and, for information, its fp32 path)
+ *   katali-hip check-attn            norm, rotation, cache store and attention of a
+ *                                    prompt and of single tokens behind it, fp32,
+ *                                    fp16 and bf16 caches, against the CPU in double
  *   katali-hip matvec-bench [reps]   dense GEMV: event-timed us per call and GB/s
- *   katali-hip bench [tokens]        48-layer top-8 MoE decode (hidden 2048, 128
- *                                    experts, ffn 768), graph-replayed
+ *   katali-hip bench [tokens [context]]
+ *                                    48-layer top-8 MoE decode (hidden 2048, 128
+ *                                    experts, ffn 768), graph-replayed; with a
+ *                                    context also each layer's norms, q/k/v and o
+ *                                    projections (32 heads of 128 over 4 key heads)
+ *                                    and attention over that many cached tokens
  *   katali-hip bench-cold [tokens]   40 layers x 256 experts (ffn 512) + shared
  *                                    expert, routing rotated every token
  *   katali-hip gguf-info FILE        a GGUF file's header, metadata and tensor
@@ -390,6 +397,270 @@ static int moe_bench(const char *name, uint32_t L, uint32_t H, uint32_t F, uint3
     return 0;
 }
 
+/* ---- attention: norm, rotation, cache store, softmax over the cache -------- */
+#define F16 KATALI_HIP_TYPE_F16
+#define BF16 KATALI_HIP_TYPE_BF16
+
+static float cache_value(uint32_t type, const void *p, size_t i) {
+    if (type == F16) return kh_cpu_half_to_float(((const uint16_t *)p)[i]);
+    if (type == KATALI_HIP_TYPE_F32) return ((const float *)p)[i];
+    const uint32_t u = (uint32_t)((const uint16_t *)p)[i] << 16;
+    float f;
+    memcpy(&f, &u, 4);
+    return f;
+}
+
+/* Two sequences through kv_append and attention, `rows` new rows each per
+ * step, against the CPU in double. The CPU attends over the caches as the
+ * device rounded them and over its own q, so the bar is that of fp32 sums:
+ * q to 16 * 2^-24 of its largest value, outputs to rel_L2 1e-5. PASS also
+ * needs every stored value within half a step of the cache's type (plus q's
+ * bar) of the CPU's. */
+static int check_attn(uint32_t type, uint32_t dim, uint32_t heads, uint32_t kv) {
+    const uint32_t cap = 96, S = 2, steps[3] = {61, 1, 1}, eb = type == KATALI_HIP_TYPE_F32 ? 4 : 2;
+    const double base = 1e6, eps = 1e-6, scale = (float)(1.0 / sqrt((double)dim));
+    const uint64_t stride = (uint64_t)kv * dim, cache = (uint64_t)S * cap * stride;
+    const double half_step = type == F16 ? 4.8828125e-4 : type == BF16 ? 3.90625e-3 : 5.9604645e-8;
+    void *kc = NULL, *vc = NULL;
+    CK(api->malloc_(&kc, cache * eb));
+    CK(api->malloc_(&vc, cache * eb));
+    CK(api->memset_(kc, 0, cache * eb));
+    CK(api->memset_(vc, 0, cache * eb));
+    float *qw = dalloc_f(dim), *kw = dalloc_f(dim);
+    CK(api->synth_normal(qw, dim, 71, 1.0f));
+    CK(api->synth_normal(kw, dim, 72, 1.0f));
+    float *hqw = malloc(dim * 4), *hkw = malloc(dim * 4), *hk = malloc(cache * 4), *hv = malloc(cache * 4);
+    void *raw = malloc(cache * eb);
+    CK(api->download(hqw, qw, dim * 4));
+    CK(api->download(hkw, kw, dim * 4));
+    double worst = 0, worst_q = 0, worst_kv = 0;
+    uint32_t have = 0;
+    for (int st = 0; st < 3; st++) {
+        const uint32_t n = steps[st], R = n * S;
+        have += n;
+        const size_t nq = (size_t)R * heads * dim, nk = (size_t)R * stride;
+        float *q = dalloc_f(nq), *k = dalloc_f(nk), *v = dalloc_f(nk), *o = dalloc_f(nq);
+        int32_t start[3] = {0, (int32_t)n, (int32_t)R}, len[2] = {(int32_t)have, (int32_t)have};
+        void *ds = NULL, *dl = NULL;
+        CK(api->malloc_(&ds, sizeof start));
+        CK(api->malloc_(&dl, sizeof len));
+        CK(api->upload(ds, start, sizeof start));
+        CK(api->upload(dl, len, sizeof len));
+        CK(api->synth_normal(q, nq, 81 + 3 * st, 2.0f));
+        CK(api->synth_normal(k, nk, 82 + 3 * st, 2.0f));
+        CK(api->synth_normal(v, nk, 83 + 3 * st, 1.0f));
+        float *hq = malloc(nq * 4), *hkn = malloc(nk * 4), *hvn = malloc(nk * 4), *ho = malloc(nq * 4), *hqo = malloc(nq * 4);
+        CK(api->download(hq, q, nq * 4));
+        CK(api->download(hkn, k, nk * 4));
+        CK(api->download(hvn, v, nk * 4));
+        KataliHipAttn a;
+        memset(&a, 0, sizeof a);
+        a.struct_size = sizeof a;
+        a.kv_type = type;
+        a.n_head = heads;
+        a.n_kv_head = kv;
+        a.head_dim = dim;
+        a.n_seq = S;
+        a.n_rows = R;
+        a.max_q = n;
+        a.max_kv = cap;
+        a.causal = 1;
+        a.q_start = (const int32_t *)ds;
+        a.kv_len = (const int32_t *)dl;
+        a.kv_seq_stride = cap * stride;
+        a.kv_row_stride = stride;
+        a.kv_head_stride = dim;
+        a.scale = (float)scale;
+        KataliHipRope r;
+        memset(&r, 0, sizeof r);
+        r.struct_size = sizeof r;
+        r.n_rot = dim;
+        r.base = (float)base;
+        r.eps = (float)eps;
+        r.q_norm_w = qw;
+        r.k_norm_w = kw;
+        CK(api->kv_append(&a, &r, q, k, v, q, kc, vc));
+        CK(api->attn(&a, q, kc, vc, o));
+        CK(api->download(hqo, q, nq * 4));
+        CK(api->download(ho, o, nq * 4));
+        CK(api->download(raw, kc, cache * eb));
+        for (size_t i = 0; i < cache; i++) hk[i] = cache_value(type, raw, i);
+        CK(api->download(raw, vc, cache * eb));
+        for (size_t i = 0; i < cache; i++) hv[i] = cache_value(type, raw, i);
+        double want[256], out[256], num = 0, den = 0;
+        for (uint32_t s = 0; s < S; s++)
+            for (uint32_t t = 0; t < n; t++) {
+                const uint32_t row = s * n + t, pos = have - n + t;
+                for (uint32_t h = 0; h < kv; h++) {
+                    const size_t at = ((size_t)(s * cap + pos) * kv + h) * dim, from = ((size_t)row * kv + h) * dim;
+                    kh_cpu_head_rope(hkn + from, hkw, dim, dim, base, eps, pos, want);
+                    for (uint32_t d = 0; d < dim; d++) {
+                        const double ek = fabs(hk[at + d] - want[d]) / (half_step * fabs(want[d]) + 1e-5);
+                        const double ev = fabs(hv[at + d] - hvn[from + d]) / (half_step * fabs(hvn[from + d]) + 1e-7);
+                        worst_kv = fmax(worst_kv, fmax(ek, ev));
+                    }
+                }
+                for (uint32_t h = 0; h < heads; h++) {
+                    const size_t at = ((size_t)row * heads + h) * dim;
+                    kh_cpu_head_rope(hq + at, hqw, dim, dim, base, eps, pos, want);
+                    double top = 0;
+                    for (uint32_t d = 0; d < dim; d++) top = fmax(top, fabs(want[d]));
+                    for (uint32_t d = 0; d < dim; d++)
+                        worst_q = fmax(worst_q, fabs(hqo[at + d] - want[d]) / (16 * 5.9604645e-8 * top));
+                    const size_t kv0 = (size_t)s * cap * stride + (size_t)(h / (heads / kv)) * dim;
+                    kh_cpu_attn_row(want, hk + kv0, hv + kv0, pos + 1, stride, dim, scale, out);
+                    for (uint32_t d = 0; d < dim; d++) {
+                        num += (ho[at + d] - out[d]) * (ho[at + d] - out[d]);
+                        den += out[d] * out[d];
+                    }
+                }
+            }
+        worst = fmax(worst, sqrt(num / den));
+        void *bufs[] = {q, k, v, o, ds, dl};
+        for (size_t i = 0; i < sizeof bufs / sizeof bufs[0]; i++) api->free_(bufs[i]);
+        free(hq); free(hkn); free(hvn); free(ho); free(hqo);
+    }
+    const int ok = worst <= 1e-5 && worst_q <= 1 && worst_kv <= 1;
+    printf("check-attn %s caches, %u heads of %u over %u: rel_L2(attention) = %.3e (<= 1e-5), q %.2f and stored values "
+           "%.2f of their bars %s\n", type == F16 ? "fp16" : type == BF16 ? "bf16" : "fp32", heads, dim, kv, worst,
+           worst_q, worst_kv, ok ? "PASS" : "FAIL");
+    void *bufs[] = {kc, vc, qw, kw};
+    for (size_t i = 0; i < sizeof bufs / sizeof bufs[0]; i++) api->free_(bufs[i]);
+    free(hqw); free(hkw); free(hk); free(hv); free(raw);
+    return ok ? 0 : 1;
+}
+
+static int cmd_check_attn(void) {
+    int fails = 0;
+    const uint32_t types[3] = {KATALI_HIP_TYPE_F32, F16, BF16};
+    for (int t = 0; t < 3; t++) {
+        fails += check_attn(types[t], 128, 32, 4);
+        fails += check_attn(types[t], 64, 6, 2);
+        fails += check_attn(types[t], 256, 16, 2);
+    }
+    return fails ? 1 : 0;
+}
+
+/* One decode token through L whole layers behind `context` cached tokens, one
+ * graph: x += y, norm, q/k/v, the new row stored, attention, o, x += o, norm,
+ * router, the MoE layer. */
+static int token_bench(uint32_t L, uint32_t H, uint32_t F, uint32_t E, uint32_t K, int tokens, uint32_t context) {
+    const uint32_t heads = 32, kv = 4, dim = 128, QR = heads * dim, KR = kv * dim;
+    const uint64_t rbg = row_bytes(Q4K, H), rbd = row_bytes(Q6K, F), cache = (uint64_t)context * KR;
+    struct layer {
+        void *g, *u, *d, *wq, *wk, *wv, *wo, *kc, *vc;
+        float *n1, *n2, *router;
+    } *w = calloc(L, sizeof *w);
+    for (uint32_t l = 0; l < L; l++) {
+        struct { void **p; uint32_t type; uint64_t rows, cols; } m[7] = {
+            {&w[l].g, Q4K, (uint64_t)E * F, H}, {&w[l].u, Q4K, (uint64_t)E * F, H}, {&w[l].d, Q6K, (uint64_t)E * H, F},
+            {&w[l].wq, Q4K, QR, H}, {&w[l].wk, Q4K, KR, H}, {&w[l].wv, Q6K, KR, H}, {&w[l].wo, Q4K, H, QR}};
+        for (int i = 0; i < 7; i++) {
+            CK(api->malloc_(m[i].p, m[i].rows * row_bytes(m[i].type, m[i].cols)));
+            /* super-block scales that give each matrix about 1/sqrt(cols) deviation */
+            const float sigma = (float)(1.0 / ((m[i].type == Q4K ? 322.0 : 1366.0) * sqrt((double)m[i].cols)));
+            CK(api->synth_fill(m[i].type, *m[i].p, m[i].rows * m[i].cols / 256, 2000 + 16 * l + i, sigma));
+        }
+        CK(api->malloc_(&w[l].kc, cache * 2));
+        CK(api->malloc_(&w[l].vc, cache * 2));
+        CK(api->memset_(w[l].kc, 0x2c, cache * 2));   /* fp16 0.0655: what earlier tokens left does not matter here */
+        CK(api->memset_(w[l].vc, 0x2c, cache * 2));
+        w[l].n1 = dalloc_f(H);
+        w[l].n2 = dalloc_f(H);
+        w[l].router = dalloc_f((size_t)E * H);
+        CK(api->synth_normal(w[l].n1, H, 2008 + 16 * l, 1.0f));
+        CK(api->synth_normal(w[l].n2, H, 2009 + 16 * l, 1.0f));
+        CK(api->synth_normal(w[l].router, (size_t)E * H, 2010 + 16 * l, (float)(1.0 / sqrt((double)H))));
+    }
+    float *x = dalloc_f(H), *xn = dalloc_f(H), *y = dalloc_f(H), *q = dalloc_f(QR), *k = dalloc_f(KR), *v = dalloc_f(KR),
+          *ao = dalloc_f(QR), *logits = dalloc_f(E), *qw = dalloc_f(dim), *kw = dalloc_f(dim);
+    CK(api->synth_normal(x, H, 5, 8.0f));
+    CK(api->synth_normal(y, H, 6, 1.0f));
+    CK(api->synth_normal(qw, dim, 7, 1.0f));
+    CK(api->synth_normal(kw, dim, 8, 1.0f));
+    void *len = NULL;
+    const int32_t hlen = (int32_t)context;
+    CK(api->malloc_(&len, 4));
+    CK(api->upload(len, &hlen, 4));
+    KataliHipAttn a;
+    memset(&a, 0, sizeof a);
+    a.struct_size = sizeof a;
+    a.kv_type = F16;
+    a.n_head = heads;
+    a.n_kv_head = kv;
+    a.head_dim = dim;
+    a.n_seq = a.n_rows = a.max_q = 1;
+    a.max_kv = context;
+    a.causal = 1;
+    a.kv_len = (const int32_t *)len;
+    a.kv_seq_stride = cache;
+    a.kv_row_stride = KR;
+    a.kv_head_stride = dim;
+    a.scale = 0.0883883f;
+    KataliHipRope r;
+    memset(&r, 0, sizeof r);
+    r.struct_size = sizeof r;
+    r.n_rot = dim;
+    r.base = 1e6f;
+    r.eps = 1e-6f;
+    r.q_norm_w = qw;
+    r.k_norm_w = kw;
+    void *graph = NULL;
+    for (int pass = 0; pass < 2; pass++) {   /* eager once (sizes the scratch), then captured */
+        if (pass) CK(api->graph_begin());
+        for (uint32_t l = 0; l < L; l++) {
+            const uint32_t types[3] = {Q4K, Q4K, Q6K};
+            const void *ws[3] = {w[l].wq, w[l].wk, w[l].wv};
+            const uint64_t rows[3] = {QR, KR, KR};
+            float *ys[3] = {q, k, v};
+            CK(api->add_rmsnorm(x, y, 1.0f, w[l].n1, H, 1e-6f, xn));
+            CK(api->matvec_multi(3, types, ws, rows, H, xn, ys));
+            CK(api->kv_append(&a, &r, q, k, v, q, w[l].kc, w[l].vc));
+            CK(api->attn(&a, q, w[l].kc, w[l].vc, ao));
+            CK(api->matvec(Q4K, w[l].wo, H, QR, ao, y));
+            CK(api->add_rmsnorm(x, y, 1.0f, w[l].n2, H, 1e-6f, xn));
+            CK(api->matvec(KATALI_HIP_TYPE_F32, w[l].router, E, H, xn, logits));
+            KataliHipMoe m = {sizeof m, Q4K, Q4K, Q6K, H, F, E, w[l].g, w[l].u, w[l].d, NULL, NULL, NULL};
+            KataliHipMoeRoute mr;
+            memset(&mr, 0, sizeof mr);
+            mr.struct_size = sizeof mr;
+            mr.n_sel = (int32_t)K;
+            mr.logits = logits;
+            CK(api->moe_layer(&m, &mr, xn, NULL, y));
+        }
+        if (pass) CK(api->graph_end(&graph));
+        else CK(api->sync());
+    }
+    void *e0 = NULL, *e1 = NULL;
+    CK(api->event_create(&e0));
+    CK(api->event_create(&e1));
+    for (int i = 0; i < 4; i++) CK(api->graph_launch(graph));
+    CK(api->sync());
+    CK(api->event_record(e0));
+    for (int t = 0; t < tokens; t++) CK(api->graph_launch(graph));
+    CK(api->event_record(e1));
+    CK(api->sync());
+    float ms = 0;
+    CK(time_ms(e0, e1, &ms));
+    const double per_tok = ms / tokens;
+    const double bytes = (double)L * (K * (2.0 * F * rbg + H * rbd) + (QR + KR) * (double)rbg + KR * (double)row_bytes(Q6K, H) +
+                                      H * (double)row_bytes(Q4K, QR) + 4.0 * E * H + 4.0 * cache);
+    printf("bench: %u layers with attention (%u heads of %u over %u key heads, %u cached tokens, fp16), %u experts, top-%u, "
+           "hidden %u, ffn %u: %.3f ms/token, %.1f us/layer, %.1f GB/s, %.1f tok/s\n", L, heads, dim, kv, context, E, K, H, F,
+           per_tok, per_tok * 1e3 / L, bytes / (per_tok * 1e-3) / 1e9, 1e3 / per_tok);
+    api->graph_destroy(graph);
+    api->event_destroy(e0);
+    api->event_destroy(e1);
+    for (uint32_t l = 0; l < L; l++) {
+        void *bufs[] = {w[l].g, w[l].u, w[l].d, w[l].wq, w[l].wk, w[l].wv, w[l].wo, w[l].kc, w[l].vc, w[l].n1, w[l].n2, w[l].router};
+        for (size_t i = 0; i < sizeof bufs / sizeof bufs[0]; i++) api->free_(bufs[i]);
+    }
+    void *bufs[] = {x, xn, y, q, k, v, ao, logits, qw, kw, len};
+    for (size_t i = 0; i < sizeof bufs / sizeof bufs[0]; i++) api->free_(bufs[i]);
+    free(w);
+    return 0;
+}
+
 static int cmd_gguf_info(const char *path) {
     KataliHipGguf *g = NULL;
     char err[256];
@@ -516,7 +787,8 @@ static int cmd_gguf_check(const char *path) {
 }
 
 static void usage(void) {
-    fputs("usage: katali-hip info | dp4a-selftest | check | check-moe | matvec-bench [reps] | bench [tokens] |"
+    fputs("usage: katali-hip info | dp4a-selftest | check | check-moe | check-attn | matvec-bench [reps] |"
+          " bench [tokens [context]] |"
           " bench-cold [tokens] | gguf-info FILE | gguf-check FILE\n", stderr);
 }
 
@@ -537,6 +809,10 @@ int main(int argc, char **argv) {
     if (!strcmp(cmd, "check")) return cmd_check();
     if (!strcmp(cmd, "check-moe")) return cmd_check_moe();
     if (!strcmp(cmd, "matvec-bench")) return cmd_matvec_bench(n > 0 ? n : 5);
+    if (!strcmp(cmd, "check-attn")) return cmd_check_attn();
+    const int context = argc > 3 ? atoi(argv[3]) : 0;
+    if (!strcmp(cmd, "bench") && context > 0)
+        return token_bench(48, 2048, 768, 128, 8, n > 0 ? n : 32, (uint32_t)context);
     if (!strcmp(cmd, "bench")) return moe_bench("bench", 48, 2048, 768, 128, 8, 0, n > 0 ? n : 32);
     if (!strcmp(cmd, "bench-cold")) return moe_bench("bench-cold", 40, 2048, 512, 256, 8, 1, n > 0 ? n : 64);
     if (!strcmp(cmd, "gguf-check") && argc > 2) return cmd_gguf_check(argv[2]);

@@ -196,3 +196,33 @@ float kh_cpu_silu_mul(float g, float u) {
     const float den = 1.0f + lib_expf(-g);
     return g / den * u;
 }
+
+void kh_cpu_head_rope(const float *x, const float *w, uint32_t n, uint32_t n_rot, double base, double eps, int64_t pos,
+                      double *out) {
+    double ss = 0;
+    for (uint32_t i = 0; i < n; i++) ss += (double)x[i] * x[i];
+    const double inv = w ? 1.0 / sqrt(ss / n + eps) : 1.0;
+    for (uint32_t i = 0; i < n; i++) out[i] = x[i] * inv * (w ? w[i] : 1.0);
+    for (uint32_t i = 0; i < n_rot / 2; i++) {
+        const double a = (double)pos * pow(base, -2.0 * i / n_rot), c = cos(a), s = sin(a);
+        const double u = out[i], v = out[i + n_rot / 2];
+        out[i] = u * c - v * s;
+        out[i + n_rot / 2] = u * s + v * c;
+    }
+}
+
+void kh_cpu_attn_row(const double *q, const float *k, const float *v, uint64_t n, uint64_t stride, uint32_t dim,
+                     double scale, double *out) {
+    double m = -INFINITY, l = 0;
+    for (uint32_t d = 0; d < dim; d++) out[d] = 0;
+    for (uint64_t j = 0; j < n; j++) {
+        double x = 0;
+        for (uint32_t d = 0; d < dim; d++) x += q[d] * k[j * stride + d];
+        x *= scale;
+        const double mn = x > m ? x : m, f = exp(m - mn), p = exp(x - mn);
+        l = l * f + p;
+        for (uint32_t d = 0; d < dim; d++) out[d] = out[d] * f + p * v[j * stride + d];
+        m = mn;
+    }
+    for (uint32_t d = 0; d < dim; d++) out[d] = l > 0 ? out[d] / l : 0;
+}

@@ -35,4 +35,14 @@ float kh_cpu_dot_q4k_q8(const void *row, const void *q8, uint64_t nb);
  * exp256_ps, V/src/gguf_simd_x86.c:744-761), every step one fp32 rounding. */
 float kh_cpu_silu_mul(float g, float u);
 
+/* One head's values x[n] as the step before attention leaves them, in double:
+ * x / sqrt(mean(x^2) + eps) * w (w NULL: x), then values i and i + n_rot/2 of
+ * the first n_rot turned by pos * base^(-2i/n_rot). */
+void kh_cpu_head_rope(const float *x, const float *w, uint32_t n, uint32_t n_rot, double base, double eps, int64_t pos,
+                      double *out);
+/* out[dim] = softmax(scale * q . k_j) v_j over the n keys at k + j * stride,
+ * in double. */
+void kh_cpu_attn_row(const double *q, const float *k, const float *v, uint64_t n, uint64_t stride, uint32_t dim,
+                     double scale, double *out);
+
 #endif

@@ -48,6 +48,12 @@ def lib():
     (dict(kv_seq_stride=1 << 60), K.E_UNSUPPORTED),
     (dict(scale=float("nan")), K.E_INVALID), (dict(scale=float("inf")), K.E_INVALID),
     (dict(softcap=-1.0), K.E_INVALID), (dict(softcap=float("inf")), K.E_INVALID),
+    (dict(n_rows=(1 << 22) + 1, max_q=1, n_head=1, n_kv_head=1, q_start=Ptr(64)), K.E_UNSUPPORTED),
+    (dict(n_rows=1 << 22, max_q=1, n_head=1, n_kv_head=1, q_start=Ptr(64)), 0),
+    (dict(n_seq=65535, n_rows=65535, n_head=512, n_kv_head=1), K.E_UNSUPPORTED),
+    (dict(n_seq=65535, n_rows=65535, n_head=128, n_kv_head=1), 0),
+    (dict(n_seq=64, n_rows=1 << 16, max_q=1 << 15, q_start=Ptr(64)), K.E_UNSUPPORTED),
+    (dict(n_seq=64, n_rows=1 << 16, max_q=1 << 14, q_start=Ptr(64)), 0),
     (dict(n_rows=1 << 28, max_q=1 << 28, q_start=Ptr(64)), K.E_UNSUPPORTED),
     (dict(n_seq=65535, n_rows=1 << 20, max_q=1 << 20, q_start=Ptr(64)), K.E_UNSUPPORTED),
 ])

@@ -45,6 +45,22 @@ def test_bench_reports_a_rate():
     assert "GB/s" in p.stdout and "tok/s" in p.stdout
 
 
+@pytest.mark.gpu
+def test_check_attn_passes():
+    """Norm, rotation, cache store and attention against the CPU, nine shapes."""
+    p = run("check-attn")
+    assert p.returncode == 0, p.stdout + p.stderr
+    assert p.stdout.count("PASS") == 9 and "FAIL" not in p.stdout
+
+
+@pytest.mark.gpu
+def test_bench_with_a_context():
+    """A decode token through whole layers, attention over cached tokens included."""
+    p = run("bench", "2", "300")
+    assert p.returncode == 0, p.stderr
+    assert "300 cached tokens" in p.stdout and "tok/s" in p.stdout
+
+
 def test_gguf_info(tmp_path):
     """gguf-info reads a file's table without a GPU."""
     from gguf_models import build_gguf

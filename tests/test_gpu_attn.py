@@ -361,3 +361,63 @@ def test_steps_of_a_chain(hip):
         assert np.abs(c["q"] - want_q).max() <= 2.0 ** -19 * np.abs(want_q).max()
         O.compare(c, o.download(np.float32).reshape(c["q"].shape), O.attn(c))
         k, v = c["k"], c["v"]
+
+
+def test_another_stream(hip):
+    """The calls run on the stream that set_stream names, in order with its other work."""
+    import ctypes as C
+    with open("/proc/self/maps") as f:   # the HIP runtime that the library loaded
+        runtime = C.CDLL(next(line.split()[-1] for line in f if "libamdhip64" in line))
+    rng = np.random.default_rng(17)
+    c = O.make(rng, 3, [1, 1, 1], [400, 30, 1], 400, 8, 2, 128, K.F16)
+    want, keep = O.attn(c), []
+    O.run(hip, c, keep_out=keep)
+    d, q, k, v, o = keep
+    s = C.c_void_p()
+    assert runtime.hipStreamCreateWithFlags(C.byref(s), 1) == 0
+    hip.check(hip.lib.katali_hip_set_stream(s))
+    try:
+        for _ in range(3):
+            hip.memset(o, 0, o.nbytes)
+            hip.attn(d, q, k, v, o)
+        O.compare(c, o.download(np.float32).reshape(3, 8, 128), want)
+    finally:
+        hip.check(hip.lib.katali_hip_set_stream(None))
+        assert runtime.hipStreamDestroy(s) == 0
+
+
+def test_first_call_inside_a_capture():
+    """In a fresh process: the first attention call allocates the scratch, so
+    inside a capture it is refused; after one eager call it may be captured."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = (
+        "import numpy as np, sys\n"
+        "import attn_oracle as O, katali_hip as K\n"
+        "hip = K.KataliHip(); assert hip.probe()\n"
+        "c = O.make(np.random.default_rng(0), 1, [1], [300], 300, 4, 1, 64, K.F32)\n"
+        "i32 = lambda a: hip.to_device(np.asarray(a, np.int32))\n"
+        "d = hip.attn_desc(K.F32, 4, 1, 64, n_seq=1, kv_len=i32([300]), max_kv=300, kv_seq_stride=19200,\n"
+        "                  kv_row_stride=64, kv_head_stride=64, scale=c['scale'])\n"
+        "q, k, v, o = hip.to_device(c['q']), hip.to_device(c['k_raw']), hip.to_device(c['v_raw']), hip.alloc(1024)\n"
+        "hip.graph_begin()\n"
+        "try:\n"
+        "    hip.attn(d, q, k, v, o); sys.exit('not refused')\n"
+        "except K.HipError as e:\n"
+        "    assert e.rc == K.E_INVALID and 'capture' in str(e), e\n"
+        "try:\n"
+        "    hip.graph_destroy(hip.graph_end())\n"
+        "except K.HipError:\n"
+        "    pass\n"
+        "hip.attn(d, q, k, v, o)\n"
+        "hip.graph_begin(); hip.attn(d, q, k, v, o); g = hip.graph_end()\n"
+        "for _ in range(3):\n"
+        "    hip.memset(o, 0, 1024); hip.graph_launch(g)\n"
+        "    got = o.download(np.float32).reshape(1, 4, 64)\n"
+        "    O.compare(c, got, O.attn(c))\n"
+        "hip.graph_destroy(g); print('fine')\n")
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100,
+                       env={**os.environ, "PYTHONPATH": os.pathsep.join([here, os.path.join(here, "..", "katali-lab_amd")])})
+    assert p.returncode == 0 and "fine" in p.stdout, p.stdout + p.stderr
