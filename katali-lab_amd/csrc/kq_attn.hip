@@ -606,8 +606,10 @@ __device__ __forceinline__ Item make_item(const AttnArgs &a, uint32_t id) {
     id /= a.n_kv;
     it.split = id % splits;
     id /= splits;
-    it.tile = tiles - 1 - id % tiles;   // later rows see more keys: they start first
-    it.seq = id / tiles;
+    // later rows see more keys: they start first, in all sequences
+    const uint32_t seqs = it.pooled ? 1 : a.n_seq;
+    it.seq = id % seqs;
+    it.tile = tiles - 1 - id / seqs;
     return it;
 }
 

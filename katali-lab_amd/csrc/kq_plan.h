@@ -108,7 +108,7 @@ inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint3
     const uint32_t cap = most_slots < ATTN_MAX_SLOTS ? (uint32_t)most_slots : ATTN_MAX_SLOTS;
     const uint32_t waves = 4;                               // ROWS_WAVES
     const uint32_t few = waves * (f32 ? 16 : 32);           // a tile of keys for every wave
-    const uint32_t many = f32 ? 128 : 256;                  // four to eight stages
+    const uint32_t many = f32 ? 64 : 128;                  // two stages or more
     auto cover = [](uint64_t n, uint64_t by) { return (n + by - 1) / by; };
     // parts for `items` items of up to `keys` keys each, so that about `want` workgroups come of it;
     // a part has at least `least` keys, and shorter items take fewer parts of the same length
