@@ -236,33 +236,24 @@ struct Frag {
 
     // rows j0 ..; rows from `end` on repeat the last one before it: their
     // scores are masked, their values weigh zero and are some row's own
-    __device__ __forceinline__ void load(const char *kb, const char *vb, uint32_t row_bytes, int32_t j0, int32_t end,
-                                         int lane) {
+    __device__ __forceinline__ void load_keys(const char *base, uint32_t row_bytes, int32_t j0, int32_t end, int lane) {
         const uint32_t c = lane & 15, g = lane >> 4;
-        const uint64_t at = (uint64_t)(uint32_t)j0 * row_bytes;
-        const char *kp = kb + at, *vp = vb + at;
+        const char *p = base + (uint64_t)(uint32_t)j0 * row_bytes + g * 16;
         const int32_t n = end - j0;
-        if (n >= G::KT) {
-            const uint32_t ko = c * row_bytes + g * 16, vo = 4 * g * row_bytes + c * (G::DPL * G::EB);
 #pragma unroll
-            for (int t = 0; t < G::KR; t++)
+        for (int t = 0; t < G::KR; t++) {
+            const uint32_t off = (uint32_t)min((int32_t)c + 16 * t, n - 1) * row_bytes;
 #pragma unroll
-                for (int i = 0; i < G::KC; i++)
-                    k[t][i] = *(const uint4 *)(kp + (uint64_t)t * 16 * row_bytes + ko + i * 64);
-#pragma unroll
-            for (int r = 0; r < G::VR; r++) ldv(r, vp + (uint64_t)((r & 3) + (r >> 2) * 16) * row_bytes + vo);
-        } else {
-#pragma unroll
-            for (int t = 0; t < G::KR; t++) {
-                const uint32_t ko = (uint32_t)min((int32_t)c + 16 * t, n - 1) * row_bytes + g * 16;
-#pragma unroll
-                for (int i = 0; i < G::KC; i++) k[t][i] = *(const uint4 *)(kp + ko + i * 64);
-            }
-#pragma unroll
-            for (int r = 0; r < G::VR; r++)
-                ldv(r, vp + (uint32_t)min((int32_t)(4 * g) + (r & 3) + (r >> 2) * 16, n - 1) * row_bytes +
-                           c * (G::DPL * G::EB));
+            for (int i = 0; i < G::KC; i++) k[t][i] = *(const uint4 *)(p + off + i * 64);
         }
+    }
+    __device__ __forceinline__ void load_values(const char *base, uint32_t row_bytes, int32_t j0, int32_t end, int lane) {
+        const uint32_t c = lane & 15, g = lane >> 4;
+        const char *p = base + (uint64_t)(uint32_t)j0 * row_bytes + c * (G::DPL * G::EB);
+        const int32_t n = end - j0;
+#pragma unroll
+        for (int r = 0; r < G::VR; r++)
+            ldv(r, p + (uint32_t)min((int32_t)(4 * g) + (r & 3) + (r >> 2) * 16, n - 1) * row_bytes);
     }
     __device__ __forceinline__ uint4 key(int t, int i) const { return k[t][i]; }
     // V^T's operand for columns DPL (l % 16) + t: halves of 4 + 4 rows exchanged
@@ -432,10 +423,10 @@ __device__ __forceinline__ void ahead(uint4 (&r)[A + 1], Load load, Use use) {
 }
 
 // One tile of keys for a wave's B blocks of 16 rows: every operand piece of K
-// and V is taken once for all of them.
-template <int TY, int D, int B, class Query, class Src>
-__device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Query (&q)[B], const Src &f, const Row (&row)[B],
-                                          int32_t j0, int32_t end, const bool (&whole)[B], int lane) {
+// and V is taken once for all of them. keys_done: called when K's are used up.
+template <int TY, int D, int B, class Query, class Src, class Then>
+__device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Query (&q)[B], Src &f, const Row (&row)[B],
+                                          int32_t j0, int32_t end, const bool (&whole)[B], int lane, Then keys_done) {
     using G = Tile<TY, D>;
     constexpr int NT = TERMS<TY>, KR = Src::KR, VR = 4 * KR;
     constexpr int A = TY == ATTN_BF16 && D == 256 ? 1 : 2;   // 1: registers
@@ -477,6 +468,7 @@ __device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Query (&
         for (int b = 0; b < B; b++)
 #pragma unroll
             for (int r = 0; r < 4; r++) y[b][4 * t + r] = s[t][b][r];
+    keys_done();
     // the first pieces of V are on their way while the weights are formed
     uint4 pre[A + 1];
     if constexpr (Src::FROM_LDS && TY != ATTN_F32) {
@@ -597,9 +589,8 @@ struct Item {
 };
 __device__ __forceinline__ Item make_item(const AttnArgs &a, uint32_t id) {
     Item it;
-    id += a.first_item;
-    it.pooled = id >= a.own_items;
-    if (it.pooled) id -= a.own_items;
+    it.pooled = id < a.shared_items;   // the longer ones first
+    if (!it.pooled) id -= a.shared_items;
     const uint32_t splits = it.pooled ? a.shared_splits : a.own_splits;
     const uint32_t tiles = it.pooled ? a.shared_tiles : a.own_tiles;
     it.kvh = id % a.n_kv;
@@ -729,6 +720,12 @@ __device__ __forceinline__ void attn_rows_item(const AttnArgs &a, const Item &it
     int32_t c0, c1;
     split_share(a, it, sp.lo, sp.hi, G::KT, c0, c1);
 
+    // a part without keys leaves word of it, and that is all
+    if (c0 >= c1 && a.slots) {
+        if (wave == 0 && lane < 16 && row.valid) a.ml[slot_of(a, row_head(a, row), it)] = make_float2(NEG_INF, 0.0f);
+        return;
+    }
+
     // the wave's first tile is asked for before q is waited for (with 256-wide
     // heads there are no registers for both)
     Segment g = segment(a, G::EB, it.kvh, it.seq, true, c0, c1);
@@ -740,23 +737,32 @@ __device__ __forceinline__ void attn_rows_item(const AttnArgs &a, const Item &it
         own = true;
     }
     Frag<TY, D> f;
-    if (D <= 128 && j < g.c1) f.load(g.k, g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
+    auto load = [&] {
+        f.load_keys(g.k, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
+        f.load_values(g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
+    };
+    if (D <= 128 && j < g.c1) load();
     Wave16<TY, D> sts[1], &st = sts[0];
     QueryLds<TY, D> q[1] = {{lds.q + lane * 16, wave, W}};
     st.init(a, row, lane, q[0]);
     __syncthreads();
-    if (D > 128 && j < g.c1) f.load(g.k, g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
+    if (D > 128 && j < g.c1) load();
     while (j < g.c1) {
         const bool whole[1] = {j >= sp.all_lo && j + G::KT <= min(sp.all_hi, g.c1)};
-        asm volatile("" ::: "memory");   // q's pieces are read again for each tile, not kept
-        attn_step<TY, D, 1>(sts, q, f, rows, j, g.c1, whole, lane);
+        const int32_t at = j, end = g.c1;
         j += W * G::KT;
         if (j >= g.c1 && !own) {
             g = segment(a, G::EB, it.kvh, it.seq, false, c0, c1);
             j = g.c0 + wave * G::KT;
             own = true;
         }
-        if (j < g.c1) f.load(g.k, g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
+        asm volatile("" ::: "memory");   // q's pieces are read again for each tile, not kept
+        // the next tile's keys are asked for when these have been used, its values behind them
+        attn_step<TY, D, 1>(sts, q, f, rows, at, end, whole, lane, [&] {
+            if (j < g.c1) f.load_keys(g.k, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
+            asm volatile("" ::: "memory");
+        });
+        if (j < g.c1) f.load_values(g.v, g.row_bytes, j - g.origin, g.c1 - g.origin, lane);
     }
     st.l = rows_sum(st.l);
     __syncthreads();   // q is done with: its LDS takes the sums
@@ -961,6 +967,12 @@ __device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it
     hi = __builtin_amdgcn_readfirstlane(hi);
     split_share(a, it, lo, hi, S::NK, c0, c1);
 
+    if (c0 >= c1 && a.slots) {   // a part without keys
+#pragma unroll
+        for (int b = 0; b < B; b++)
+            if (lane < 16 && row[b].valid) a.ml[slot_of(a, row_head(a, row[b]), it)] = make_float2(NEG_INF, 0.0f);
+        return;
+    }
     Wave16<TY, D> st[B];
     QueryRegs<TY, D> q[B];
 #pragma unroll
@@ -990,7 +1002,8 @@ __device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it
                     bool whole[B];
 #pragma unroll
                     for (int b = 0; b < B; b++) whole[b] = js >= sp[b].all_lo && js + S::SK <= min(sp[b].all_hi, g.c1);
-                    attn_step<TY, D, B>(st, q, S::view(lds.stage[at], part, lane), row, js, g.c1, whole, lane);
+                    auto view = S::view(lds.stage[at], part, lane);
+                    attn_step<TY, D, B>(st, q, view, row, js, g.c1, whole, lane, [] {});
                 }
                 if (jn < g.c1) stage.store(lds.stage[at ^ 1], part);
             }
@@ -1110,9 +1123,8 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
 }
 
 template <int TY, int D>
-static hipError_t attn_run(AttnArgs a, const AttnPlan &p, hipStream_t s) {
+static hipError_t attn_run(const AttnArgs &a, const AttnPlan &p, hipStream_t s) {
     const dim3 rows(64 * ROWS_WAVES), tile(64 * TILE_WAVES<TY, D>);
-    a.first_item = 0;
     if (p.form == ATTN_TILES) {
         hipLaunchKernelGGL((k_attn_tile<TY, D>), dim3(p.own_items), tile, 0, s, a);
     } else if (p.form == ATTN_ROWS) {
@@ -1121,11 +1133,13 @@ static hipError_t attn_run(AttnArgs a, const AttnPlan &p, hipStream_t s) {
         hipLaunchKernelGGL((k_attn_mixed<TY, D>), dim3(p.own_items + p.shared_items), rows, 0, s, a);
     } else {
         // no registers for both in one kernel
-        hipLaunchKernelGGL((k_attn<TY, D>), dim3(p.own_items), rows, 0, s, a);
+        AttnArgs own = a, pooled = a;
+        own.shared_items = 0;
+        pooled.own_items = 0;
+        hipLaunchKernelGGL((k_attn<TY, D>), dim3(p.own_items), rows, 0, s, own);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        a.first_item = p.own_items;
-        hipLaunchKernelGGL((k_attn_tile<TY, D>), dim3(p.shared_items), tile, 0, s, a);
+        hipLaunchKernelGGL((k_attn_tile<TY, D>), dim3(p.shared_items), tile, 0, s, pooled);
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !a.slots) return e;
@@ -1143,6 +1157,7 @@ hipError_t launch_attn(AttnArgs a, uint32_t type, uint32_t head_dim, const AttnP
     a.shared_splits = p.shared_splits;
     a.slots = p.slots;
     a.own_items = p.own_items;
+    a.shared_items = p.shared_items;
     a.own_chunk = p.own_chunk;
     a.shared_chunk = p.shared_chunk;
     a.acc = (float *)scratch;
