@@ -119,12 +119,15 @@ struct Score {
     float mul;      // product -> score (with a cap: -> score / cap)
     float cap;      // cap log2(e)
     float slope;    // -slope log2(e)
+    float near;     // distance of the row's nearest key
     bool capped, sloped;
     bool bare;      // neither, and a positive factor for every row of the wave
 };
 struct Row;
 __device__ __forceinline__ Score make_score(const AttnArgs &a, const Row &r, float mul);
-// scores of the keys j0 + off(r), pos0 = position - j0
+// scores of the keys j0 + off(r), pos0 = position - j0. The bias counts from the
+// row's nearest key on, which the softmax does not notice: a row whose
+// document leaves far keys only keeps the bits of its scores.
 template <int N, class Off>
 __device__ __forceinline__ void scores(const Score &c, float (&y)[N], int32_t pos0, Off off) {
     if (c.capped) {
@@ -152,7 +155,7 @@ __device__ __forceinline__ void scores(const Score &c, float (&y)[N], int32_t po
     if (c.sloped) {
         const float p = (float)pos0;
 #pragma unroll
-        for (int r = 0; r < N; r++) y[r] = fmaf(fabsf(p - (float)off(r)), c.slope, y[r]);
+        for (int r = 0; r < N; r++) y[r] = fmaf(fabsf(p - (float)off(r)) - c.near, c.slope, y[r]);
     }
 }
 
@@ -200,6 +203,7 @@ __device__ __forceinline__ Score make_score(const AttnArgs &a, const Row &r, flo
     c.cap = a.softcap * LOG2E;
     c.mul = c.capped ? mul / a.softcap : mul * LOG2E;
     c.slope = c.sloped && r.valid ? a.slopes[r.head] * -LOG2E : 0.0f;
+    c.near = (float)max(max(r.lo - r.pos, r.pos - r.hi + 1), 0);
     c.bare = !c.capped && !c.sloped && !__any(!(c.mul > 0.0f));
     return c;
 }

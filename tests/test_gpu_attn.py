@@ -83,6 +83,18 @@ def test_documents(hip, t, causal, rows, keys):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("rows,shared", [(1, 0), (1, 900), (50, 0)])
+def test_bias_of_rows_that_see_far_keys_only(hip, t, rows, shared):
+    """Rows whose documents end far before them: biases of several hundred,
+    the same for all their keys but for a few units, cost no bits."""
+    rng = np.random.default_rng(21)
+
+    def far(c):
+        return np.zeros(c["n_rows"], int), np.asarray([40 + 3 * (i % 9) for i in range(c["n_rows"])])
+    check(hip, O.make(rng, 3, [rows] * 3, [1000, 800, 900], 1000, 8, 2, 128, t, alibi=True, docs=far, n_shared=shared))
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
 @pytest.mark.parametrize("prefix", [[0, 30, 2 ** 31 - 1], [-5, 61, 100]])
 def test_prefix_seen_from_both_sides(hip, t, prefix):
     rng = np.random.default_rng(2)
