@@ -259,16 +259,17 @@ struct Frag {
         for (int r = 0; r < G::VR; r++)
             ldv(r, p + (uint32_t)min((int32_t)(4 * g) + (r & 3) + (r >> 2) * 16, n - 1) * row_bytes);
     }
-    __device__ __forceinline__ uint4 key(int t, int i) const { return k[t][i]; }
+    static constexpr int PLANES = 1;
+    __device__ __forceinline__ uint4 key(int t, int i, int) const { return k[t][i]; }
     // V^T's operand for columns DPL (l % 16) + t: halves of 4 + 4 rows exchanged
-    __device__ __forceinline__ uint4 value(int t) const {
+    __device__ __forceinline__ uint4 value(int t, int) const {
         const uint32_t sel = t & 1 ? 0x07060302u : 0x05040100u;
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) w[i] = __builtin_amdgcn_perm(v[2 * i + 1][t / 2], v[2 * i][t / 2], sel);
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
-    __device__ __forceinline__ float value(int r, int t) const { return __uint_as_float(v[r][t]); }
+    __device__ __forceinline__ float value32(int r, int t) const { return __uint_as_float(v[r][t]); }
     __device__ __forceinline__ void ldv(int r, const char *p) {
         if constexpr (G::VW >= 4) {
 #pragma unroll
@@ -434,16 +435,19 @@ __device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Query (&
     using G = Tile<TY, D>;
     constexpr int NT = TERMS<TY>, KR = Src::KR, VR = 4 * KR;
     constexpr int A = TY == ATTN_BF16 && D == 256 ? 1 : 2;   // 1: registers
+    constexpr int PL = Src::PLANES;
     float y[B][VR];
     f32x4 s[KR][B];
 #pragma unroll
     for (int t = 0; t < KR; t++)
 #pragma unroll
         for (int b = 0; b < B; b++) s[t][b] = f32x4{0, 0, 0, 0};
+    // piece i: neighbours add to different sums; of a value in terms itself, term
+    // p meets the terms 0 .. NT-1-p of the other side: what is left out is below 2^-24
     auto product = [&](int i, const uint4 &k) {
-        const int c = i / KR, t = i % KR;   // neighbours add to different sums
+        const int t = i % KR, p = i / KR % PL, c = i / KR / PL;
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NT - p; n++)
 #pragma unroll
             for (int b = 0; b < B; b++) {
                 if constexpr (TY == ATTN_F32) {
@@ -456,15 +460,16 @@ __device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Query (&
                 }
             }
     };
-    constexpr int NK = KR * G::KC;
+    constexpr int NK = KR * PL * G::KC;
+    auto key = [&](int i) { return f.key(i % KR, i / KR / PL, i / KR % PL); };
     if constexpr (Src::FROM_LDS && TY != ATTN_F32) {
         uint4 r[A + 1];
 #pragma unroll
-        for (int i = 0; i < A; i++) r[i] = f.key(i % KR, i / KR);
-        ahead<NK, A>(r, [&](int i) { return f.key(i % KR, i / KR); }, product);
+        for (int i = 0; i < A; i++) r[i] = key(i);
+        ahead<NK, A>(r, key, product);
     } else {
 #pragma unroll
-        for (int i = 0; i < NK; i++) product(i, f.key(i % KR, i / KR));
+        for (int i = 0; i < NK; i++) product(i, key(i));
     }
 #pragma unroll
     for (int t = 0; t < KR; t++)
@@ -477,7 +482,7 @@ __device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Query (&
     uint4 pre[A + 1];
     if constexpr (Src::FROM_LDS && TY != ATTN_F32) {
 #pragma unroll
-        for (int i = 0; i < A; i++) pre[i] = f.value(i);
+        for (int i = 0; i < A; i++) pre[i] = f.value(i / PL, i % PL);
         asm volatile("" ::: "memory");
     }
 #pragma unroll
@@ -487,7 +492,7 @@ __device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Query (&
         for (int r = 0; r < VR; r++)
 #pragma unroll
             for (int t = 0; t < G::DPL; t++) {
-                const float v = f.value(r, t);
+                const float v = f.value32(r, t);
 #pragma unroll
                 for (int b = 0; b < B; b++)
                     st[b].o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, y[b][r], st[b].o[t], 0, 0, 0);
@@ -498,18 +503,19 @@ __device__ __forceinline__ void attn_step(Wave16<TY, D> (&st)[B], const Query (&
         for (int b = 0; b < B; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++) split<TY>(y[b][2 * i], y[b][2 * i + 1], pt[b][i]);
-        auto add = [&](int t, const uint4 &vt) {
+        auto add = [&](int i, const uint4 &vt) {
+            const int t = i / PL, p = i % PL;
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int n = 0; n < NT - p; n++)
 #pragma unroll
                 for (int b = 0; b < B; b++)
                     st[b].o[t] = mfma32<TY>(vt, make_uint4(pt[b][0][n], pt[b][1][n], pt[b][2][n], pt[b][3][n]), st[b].o[t]);
         };
         if constexpr (Src::FROM_LDS) {
-            ahead<G::DPL, A>(pre, [&](int t) { return f.value(t); }, add);
+            ahead<G::DPL * PL, A>(pre, [&](int i) { return f.value(i / PL, i % PL); }, add);
         } else {
 #pragma unroll
-            for (int t = 0; t < G::DPL; t++) add(t, f.value(t));
+            for (int t = 0; t < G::DPL; t++) add(t, f.value(t, 0));
         }
     }
 }
@@ -664,9 +670,9 @@ __device__ __forceinline__ void split_share(const AttnArgs &a, const Item &it, i
 }
 
 // Rows of the wave that met an infinity or NaN, key by key; buf: D floats of LDS of the wave's own.
-template <int TY, int D, int W>
+template <int TY, int D, int W, int CT>
 __device__ __forceinline__ void odd_rows(const AttnArgs &a, const Item &it, const Row &row, int32_t c0, int32_t c1,
-                                         int wave, int lane, Wave16<TY, D> &st, float *buf) {
+                                         int wave, int lane, Wave16<CT, D> &st, float *buf) {
     using G = Tile<TY, D>;
     uint64_t odd = __ballot(row.valid && st.odd());
     odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xFFFF;
@@ -913,11 +919,11 @@ struct Stage {
     // the operands of one of its tiles, as Frag gives them
     struct View {
         static constexpr bool FROM_LDS = true;
-        static constexpr int KR = SK / 16;
+        static constexpr int KR = SK / 16, PLANES = 1;
         const char *kp, *vp;
-        __device__ __forceinline__ uint4 key(int t, int i) const { return *(const uint4 *)(kp + t * 16 * KROW + i * 64); }
-        __device__ __forceinline__ uint4 value(int t) const { return *(const uint4 *)(vp + t * 1024); }
-        __device__ __forceinline__ float value(int r, int t) const { return *(const float *)(vp + ((r >> 2) * 16 + (r & 3)) * KROW + t * 4); }
+        __device__ __forceinline__ uint4 key(int t, int i, int) const { return *(const uint4 *)(kp + t * 16 * KROW + i * 64); }
+        __device__ __forceinline__ uint4 value(int t, int) const { return *(const uint4 *)(vp + t * 1024); }
+        __device__ __forceinline__ float value32(int r, int t) const { return *(const float *)(vp + ((r >> 2) * 16 + (r & 3)) * KROW + t * 4); }
     };
     static __device__ __forceinline__ View view(const char *lds, int sub, int lane) {
         View w;
@@ -929,18 +935,108 @@ struct Stage {
     }
 };
 
+// fp32 keys and values in LDS as three bf16 terms each (all 24 bits), laid out
+// as Stage's 16-bit ones, a plane for each term: six bf16 products for one of
+// fp32 take 6/16 of its time on the matrix units.
+template <int D, int NTHREADS>
+struct StageTerms {
+    using G = Tile<ATTN_BF16, D>;
+    static constexpr int NK = 32, FK = 32, PARTS = 1, SK = 32;
+    static constexpr int KROW = D * 2 + 16, KPLANE = NK * KROW, VPLANE = NK * D * 2;
+    static constexpr int BYTES = 3 * (KPLANE + VPLANE);
+    static constexpr int PER_ROW = D / 4;                                     // 16-byte pieces of a row
+    static constexpr int KN = FK * PER_ROW / NTHREADS;                        // pieces of K per thread
+    static constexpr int UNITS = FK / 4 * (D / 4);                            // 4 x 4 blocks of V
+    static_assert(FK * PER_ROW % NTHREADS == 0 && UNITS <= NTHREADS, "K in whole pieces, V in one block per thread");
+
+    f32x4 k[KN], v[4];
+
+    __device__ __forceinline__ void fetch(const char *kb, const char *vb, uint32_t row_bytes, int32_t j0, int32_t end) {
+        const uint64_t at = (uint64_t)(uint32_t)j0 * row_bytes;
+        const char *kp = kb + at, *vp = vb + at;
+        const uint32_t last = (uint32_t)min(end - j0, FK) - 1;
+#pragma unroll
+        for (int n = 0; n < KN; n++) {
+            const uint32_t id = threadIdx.x + NTHREADS * n;
+            k[n] = *(const f32x4 *)(kp + (min(id / PER_ROW, last) * row_bytes + id % PER_ROW * 16));
+        }
+        if (threadIdx.x < UNITS) {
+            const uint32_t rows = threadIdx.x / (D / 4) * 4, col = threadIdx.x % (D / 4) * 16;
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] = *(const f32x4 *)(vp + (min(rows + r, last) * row_bytes + col));
+        }
+    }
+    __device__ __forceinline__ void store(char *lds, int) const {
+#pragma unroll
+        for (int n = 0; n < KN; n++) {
+            const uint32_t id = threadIdx.x + NTHREADS * n;
+            char *p = lds + id / PER_ROW * KROW + id % PER_ROW * 8;
+            uint32_t lo[3], hi[3];
+            split<ATTN_BF16>(k[n][0], k[n][1], lo);
+            split<ATTN_BF16>(k[n][2], k[n][3], hi);
+#pragma unroll
+            for (int t = 0; t < 3; t++) *(uint2 *)(p + t * KPLANE) = make_uint2(lo[t], hi[t]);
+        }
+        if (threadIdx.x < UNITS) {
+            const uint32_t q = threadIdx.x / (D / 4), col = threadIdx.x % (D / 4) * 4;
+            const uint32_t half = q / 4, lane0 = q % 4 * 16 + col / G::DPL, t0 = col % G::DPL;
+            char *p = lds + 3 * KPLANE + (t0 * 64 + lane0) * 16 + half * 8;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                uint32_t lo[3], hi[3];
+                split<ATTN_BF16>(v[0][e], v[1][e], lo);
+                split<ATTN_BF16>(v[2][e], v[3][e], hi);
+#pragma unroll
+                for (int t = 0; t < 3; t++) *(uint2 *)(p + t * VPLANE + e * 1024) = make_uint2(lo[t], hi[t]);
+            }
+        }
+    }
+    struct View {
+        static constexpr bool FROM_LDS = true;
+        static constexpr int KR = SK / 16, PLANES = 3;
+        const char *kp, *vp;
+        __device__ __forceinline__ uint4 key(int t, int i, int p) const {
+            return *(const uint4 *)(kp + p * KPLANE + t * 16 * KROW + i * 64);
+        }
+        __device__ __forceinline__ uint4 value(int t, int p) const { return *(const uint4 *)(vp + p * VPLANE + t * 1024); }
+    };
+    static __device__ __forceinline__ View view(const char *lds, int, int lane) {
+        View w;
+        w.kp = lds + (lane & 15) * KROW + (lane >> 4) * 16;
+        w.vp = lds + 3 * KPLANE + lane * 16;
+        return w;
+    }
+};
+// How a tile's keys are staged, and the type its products are formed in.
+template <int TY, int D, int NTHREADS>
+struct Staging {
+    static constexpr int CT = TY;
+    using S = Stage<TY, D, NTHREADS>;
+};
+template <int NTHREADS>
+struct Staging<ATTN_F32, 64, NTHREADS> {
+    static constexpr int CT = ATTN_BF16;
+    using S = StageTerms<64, NTHREADS>;
+};
+template <int NTHREADS>
+struct Staging<ATTN_F32, 128, NTHREADS> {
+    static constexpr int CT = ATTN_BF16;
+    using S = StageTerms<128, NTHREADS>;
+};
+
 // Many rows: the waves of a workgroup, 16 B rows each, walk the same keys,
 // staged through LDS for all of them (two buffers: the next keys are on their
 // way from memory while these are worked on, one barrier per stage).
 template <int TY, int D, int B, int W>
 struct TileLds {
-    char stage[2][Stage<TY, D, 64 * W>::BYTES];
+    char stage[2][Staging<TY, D, 64 * W>::S::BYTES];
     int32_t span[2][W];
 };
 template <int TY, int D, int B, int W>
 __device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it, char *shared) {
     using G = Tile<TY, D>;
-    using S = Stage<TY, D, 64 * W>;
+    using S = typename Staging<TY, D, 64 * W>::S;
+    constexpr int CT = Staging<TY, D, 64 * W>::CT;
     constexpr int ROWS = 16 * B * W;
     auto &lds = *(TileLds<TY, D, B, W> *)shared;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -977,8 +1073,8 @@ __device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it
             if (lane < 16 && row[b].valid) a.ml[slot_of(a, row_head(a, row[b]), it)] = make_float2(NEG_INF, 0.0f);
         return;
     }
-    Wave16<TY, D> st[B];
-    QueryRegs<TY, D> q[B];
+    Wave16<CT, D> st[B];
+    QueryRegs<CT, D> q[B];
 #pragma unroll
     for (int b = 0; b < B; b++) st[b].init(a, row[b], lane, q[b]);
     S stage;
@@ -1007,7 +1103,7 @@ __device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it
 #pragma unroll
                     for (int b = 0; b < B; b++) whole[b] = js >= sp[b].all_lo && js + S::SK <= min(sp[b].all_hi, g.c1);
                     auto view = S::view(lds.stage[at], part, lane);
-                    attn_step<TY, D, B>(st, q, view, row, js, g.c1, whole, lane, [] {});
+                    attn_step<CT, D, B>(st, q, view, row, js, g.c1, whole, lane, [] {});
                 }
                 if (jn < g.c1) stage.store(lds.stage[at ^ 1], part);
             }
@@ -1055,7 +1151,7 @@ __global__ void __launch_bounds__(64 * ROWS_WAVES, D == 64 ? (TY == ATTN_BF16 ? 
 }
 // (eight waves where four would need more registers to stage the keys than there are)
 template <int TY, int D>
-constexpr int TILE_WAVES = TY == ATTN_BF16 && D == 256 ? 8 : 4;
+constexpr int TILE_WAVES = (TY == ATTN_BF16 && D == 256) || (TY == ATTN_F32 && D == 128) ? 8 : 4;
 template <int TY, int D>
 __global__ void __launch_bounds__((64 * TILE_WAVES<TY, D>), 2) k_attn_tile(const AttnArgs a) {
     constexpr int W = TILE_WAVES<TY, D>, B = attn_tile_rows(TY, D) / (16 * W);
@@ -1133,10 +1229,10 @@ static hipError_t attn_run(const AttnArgs &a, const AttnPlan &p, hipStream_t s) 
         hipLaunchKernelGGL((k_attn_tile<TY, D>), dim3(p.own_items), tile, 0, s, a);
     } else if (p.form == ATTN_ROWS) {
         hipLaunchKernelGGL((k_attn<TY, D>), dim3(p.own_items + p.shared_items), rows, 0, s, a);
-    } else if constexpr (D <= 128) {
+    } else if constexpr (attn_mixed(TY, D)) {
         hipLaunchKernelGGL((k_attn_mixed<TY, D>), dim3(p.own_items + p.shared_items), rows, 0, s, a);
     } else {
-        // no registers for both in one kernel
+        // no registers (256 wide) or LDS (fp32 in terms, 128 wide) for both in one kernel
         AttnArgs own = a, pooled = a;
         own.shared_items = 0;
         pooled.own_items = 0;

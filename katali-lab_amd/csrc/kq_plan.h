@@ -93,11 +93,13 @@ constexpr uint64_t ATTN_SCRATCH = 64ull << 20;   // partial results: head_dim su
 constexpr uint32_t ATTN_FEW_ROWS = 32;           // rows of a key head up to which tiles of 16 are taken
 
 constexpr int ATTN_F32 = 0, ATTN_F16 = 1, ATTN_BF16 = 30;   // cache types (ggml ids)
-// Rows of a workgroup's tile: 16 for each of four waves (bf16, 256: eight), 32 where a wave's
-// registers hold two blocks and its products are not the bound by themselves (fp32's are).
+// Rows of a workgroup's tile: 16 or 32 for each of four or eight waves, by what registers and LDS hold.
 constexpr int attn_tile_rows(int type, int head_dim) {
-    return type == ATTN_F32 || (type == ATTN_F16 && head_dim == 256) || (type == ATTN_BF16 && head_dim == 128) ? 64 : 128;
+    return (type == ATTN_F32 && head_dim != 128) || (type == ATTN_F16 && head_dim == 256) ||
+                   (type == ATTN_BF16 && head_dim == 128) ? 64 : 128;
 }
+// Whether one kernel takes a shared prefix's tiles beside the rows of each sequence, else two launches do.
+constexpr bool attn_mixed(int type, int head_dim) { return head_dim == 64 || (head_dim == 128 && type != ATTN_F32); }
 
 inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint32_t n_kv, uint32_t group,
                           uint32_t max_kv, uint32_t n_shared, uint32_t head_dim, int type, uint32_t cus) {
@@ -128,8 +130,8 @@ inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint3
     if (n_shared && n_seq > 1 && !tiles && cap >= 2) {
         const uint64_t pooled = (uint64_t)n_rows * group;
         p.form = pooled > ATTN_FEW_ROWS ? ATTN_MIXED : ATTN_ROWS;
-        // (a mixed launch's tiles are of 16 rows a wave; 256-wide heads take two launches)
-        const uint32_t wide = head_dim == 256 ? (uint32_t)attn_tile_rows(type, 256) : 16 * waves;
+        // (one launch's tiles are of 16 rows a wave)
+        const uint32_t wide = attn_mixed(type, (int)head_dim) ? 16 * waves : (uint32_t)attn_tile_rows(type, (int)head_dim);
         p.shared_tiles = (uint32_t)cover(pooled, p.form == ATTN_MIXED ? wide : 16);
         split((uint64_t)n_kv * p.shared_tiles, n_shared, 2 * cus, p.form == ATTN_MIXED ? many : few, cap / 2,
               p.shared_splits, p.shared_chunk);

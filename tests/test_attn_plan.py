@@ -22,7 +22,7 @@ static void look(unsigned S, unsigned rows, unsigned max_q, unsigned kv, unsigne
     ok = ok && (unsigned long long)S * kv * p.own_tiles * p.own_splits == p.own_items;
     ok = ok && (p.form == ATTN_TILES) == (per > ATTN_FEW_ROWS);
     if (p.shared_items) {
-        const unsigned t = p.form == ATTN_ROWS ? 16 : D == 256 ? attn_tile_rows(type, 256) : 64;
+        const unsigned t = p.form == ATTN_ROWS ? 16 : attn_mixed(type, D) ? 64 : attn_tile_rows(type, D);
         ok = ok && sh && S > 1 && p.shared_chunk >= 1 && p.slots == p.own_splits + p.shared_splits;
         ok = ok && (unsigned long long)p.shared_tiles * t >= (unsigned long long)rows * g;
         ok = ok && kv * p.shared_tiles * p.shared_splits == p.shared_items;
