@@ -10,8 +10,10 @@
 // and the outputs are fp32, and the matrix instructions take 16-bit operands
 // with 16-bit caches, so q and p are each split into 16-bit terms, two of fp16
 // (22 bits together) or three of bf16 (24), and each product is formed once per
-// term into the same fp32 accumulators: nothing is rounded to 16 bits. With
-// fp32 caches the fp32 matrix instructions are used.
+// term into the same fp32 accumulators: nothing is rounded to 16 bits. (Two
+// terms of bf16 were 2.5e-6 to 5.6e-6 off the definition in 64 bits, three are
+// 2e-7 to 1.1e-6, as an fp32 evaluation is.) fp32 caches: the fp32 matrix
+// instructions, and for many rows three bf16 terms of keys and values too.
 //
 // k_attn: a wave takes 16 rows (query rows x the heads of one key head), one
 // row per lane column of the matrix tile, and walks its keys in tiles of 32
@@ -189,8 +191,10 @@ __device__ __forceinline__ Row make_row(const AttnArgs &a, uint32_t kvh, uint32_
             if (a.prefix_len) upto = max(upto, a.prefix_len[s]);
             r.hi = min(r.hi, upto);
         }
-        if (a.doc_start) r.lo = max(r.lo, a.doc_start[r.row]);
+        // (kept within the axis, so that no sum of positions leaves 32 bits)
+        if (a.doc_start) r.lo = min(max(r.lo, a.doc_start[r.row]), (int32_t)a.n_shared + own.len);
         if (a.doc_end) r.hi = min(r.hi, a.doc_end[r.row]);
+        r.hi = max(r.hi, 0);
         if (!r.valid) r.lo = r.hi = 0;
     }
     return r;
@@ -607,10 +611,15 @@ __device__ __forceinline__ Item make_item(const AttnArgs &a, uint32_t id) {
     id /= a.n_kv;
     it.split = id % splits;
     id /= splits;
-    // later rows see more keys: they start first, in all sequences
-    const uint32_t seqs = it.pooled ? 1 : a.n_seq;
-    it.seq = id % seqs;
-    it.tile = tiles - 1 - id / seqs;
+    if (it.pooled || a.by_seq) {
+        // tiles of the same keys next to each other: the second reads them from the caches
+        it.seq = id / tiles;
+        it.tile = tiles - 1 - id % tiles;
+    } else {
+        // later rows see more keys: they start first, in all sequences
+        it.seq = id % a.n_seq;
+        it.tile = tiles - 1 - id / a.n_seq;
+    }
     return it;
 }
 
@@ -706,7 +715,10 @@ __device__ __forceinline__ void odd_rows(const AttnArgs &a, const Item &it, cons
 // Few rows: the waves of a workgroup share 16 rows and take every W-th tile of
 // the keys, straight from memory into the operands' registers. Bound by
 // memory: what counts is how many loads are in flight, so the query operand,
-// the same for all waves, lies in LDS, and its registers hold more waves.
+// the same for all waves, lies in LDS, and its registers hold more waves. One
+// token over 131072 rows of 8 x 128 fp16: 101 us, 5.3 TB/s; over 300 of fp32,
+// 7.2 us, a launch and three dependent loads (eight waves: 8.8 to 11 us, the
+// larger join in LDS).
 constexpr int ROWS_WAVES = 4;
 template <int TY, int D, int W>
 struct RowsLds {
@@ -1026,7 +1038,11 @@ struct Staging<ATTN_F32, 128, NTHREADS> {
 
 // Many rows: the waves of a workgroup, 16 B rows each, walk the same keys,
 // staged through LDS for all of them (two buffers: the next keys are on their
-// way from memory while these are worked on, one barrier per stage).
+// way from memory while these are worked on, one barrier per stage). Bound by
+// the matrix units and the weights' arithmetic by turns: 32 heads, 4096 rows
+// over 4096 keys of 128, fp16 549 us (1.0 PFLOP/s of products formed, two for
+// one), bf16 709 us (1.16 PFLOP/s, three for one), fp32 (16 heads, 2048 rows) 337 us (204
+// TFLOP/s; the fp32 instructions 560 us).
 template <int TY, int D, int B, int W>
 struct TileLds {
     char stage[2][Staging<TY, D, 64 * W>::S::BYTES];
@@ -1143,7 +1159,8 @@ __device__ __forceinline__ void attn_tile_item(const AttnArgs &a, const Item &it
 
 // The kernels. Mixed: a batch's shared prefix for the rows of all sequences
 // together (many rows) beside each sequence's own keys (few rows), in one
-// launch, so that matrix work and memory traffic overlap.
+// launch: 64 requests over a prefix of 16384 bf16 keys and up to 1024 of their
+// own 96 us; with the prefix in tiles of 16 rows too (k_attn for all) 130 us.
 template <int TY, int D>
 __global__ void __launch_bounds__(64 * ROWS_WAVES, D == 64 ? (TY == ATTN_BF16 ? 3 : 4) : D == 128 ? (TY == ATTN_F32 ? 3 : 2) : TY == ATTN_F32 ? 2 : 1) k_attn(const AttnArgs a) {
     __shared__ __align__(16) char lds[sizeof(RowsLds<TY, D, ROWS_WAVES>)];
@@ -1169,7 +1186,9 @@ __global__ void __launch_bounds__(64 * ROWS_WAVES, 2) k_attn_mixed(const AttnArg
 }
 
 // The partial sums of a row, joined: SW waves per (row, head), each every
-// SW-th slot, eight slots' loads in flight.
+// SW-th slot, eight slots' loads in flight. 2.5 us where little is to be joined
+// (a launch), 4.6 us for 64 slots of 32 rows (one wave a row, one slot after
+// another: 12 us).
 template <int D, int SW>
 __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
     constexpr int E = D / 64, U = 8;
@@ -1256,6 +1275,7 @@ hipError_t launch_attn(AttnArgs a, uint32_t type, uint32_t head_dim, const AttnP
     a.shared_tiles = p.shared_tiles;
     a.shared_splits = p.shared_splits;
     a.slots = p.slots;
+    a.by_seq = p.form != ATTN_TILES;
     a.own_items = p.own_items;
     a.shared_items = p.shared_items;
     a.own_chunk = p.own_chunk;

@@ -12,7 +12,8 @@
 // position times a small frequency leaves no bits in 32), as turns of which
 // only the fraction matters, sine and cosine kept in LDS for all heads. Every
 // head is read once and written once: bound by memory, at a single token by a
-// launch's latency.
+// launch's latency. 3600 rows of 16 + 2 + 2 heads of 256, fp16: 42 us from memory
+// (3.2 TB/s), 36 us from the cache; one row of 32 + 8 + 8 heads of 128: 4.0 us.
 #include <type_traits>
 
 #include "kq_attn.h"

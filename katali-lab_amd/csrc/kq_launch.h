@@ -307,7 +307,7 @@ struct AttnArgs {
     uint32_t causal;
     float scale, softcap;
     // the plan, set by launch_attn
-    uint32_t own_tiles, own_splits, shared_tiles, shared_splits, slots, own_items, shared_items, own_chunk, shared_chunk;
+    uint32_t own_tiles, own_splits, shared_tiles, shared_splits, slots, own_items, shared_items, own_chunk, shared_chunk, by_seq;
     float *acc;
     float2 *ml;
 };

@@ -90,8 +90,8 @@ struct AttnPlan {
 };
 constexpr uint32_t ATTN_MAX_SLOTS = 64;
 constexpr uint64_t ATTN_SCRATCH = 64ull << 20;   // partial results: head_dim sums, a maximum and a sum each
-constexpr uint32_t ATTN_FEW_ROWS = 32;           // rows of a key head up to which tiles of 16 are taken
-
+constexpr uint32_t ATTN_FEW_ROWS = 32;           // rows of a key head: up to here a sequence's rows are pooled over a shared
+                                                 // prefix, beyond it the pool takes wide tiles
 constexpr int ATTN_F32 = 0, ATTN_F16 = 1, ATTN_BF16 = 30;   // cache types (ggml ids)
 // Rows of a workgroup's tile: 16 or 32 for each of four or eight waves, by what registers and LDS hold.
 constexpr int attn_tile_rows(int type, int head_dim) {
@@ -124,11 +124,24 @@ inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint3
         const uint64_t c = cover(keys ? keys : 1, parts);
         chunk = (uint32_t)(c > least ? c : least);
     };
-    const bool tiles = per_seq > ATTN_FEW_ROWS;
+    // Tiles of 16 rows read the keys once for each tile, but start sooner and spread
+    // further: they win while the tiles times their keys are few for the CUs. Up to 16 rows
+    // there is one tile. 32 heads over 8 of 128, 256 CUs, us with tiles of 16 / of 64 and more, fp16:
+    // 64 rows over 4000 keys (512 thousand tile-keys) 30 / 39, 128 rows 47 / 45, 4 x 64 rows over
+    // 1000 keys 25 / 35, over 4000 76 / 57; fp32: 32 rows over 4000 keys 35 / 41, 64 rows 57 / 49.
+    auto few_for_cus = [&](uint64_t heads_rows, uint64_t n, uint64_t keys, uint64_t per_cu) {
+        return cover(heads_rows, 16) * n * (keys ? keys : 1) <= per_cu * 128 / head_dim * cus;
+    };
+    const uint64_t all_keys = (uint64_t)max_kv + n_shared;
+    const bool pool = n_shared && n_seq > 1 && per_seq <= ATTN_FEW_ROWS && cap >= 2;
+    const bool tiles = !pool && per_seq > 16 && !few_for_cus(per_seq, (uint64_t)n_seq * n_kv, all_keys, f32 ? 1400 : 3000);
     p.own_tiles = (uint32_t)cover(per_seq, tiles ? attn_tile_rows(type, (int)head_dim) : 16);
     const uint64_t own = (uint64_t)p.own_tiles * n_seq * n_kv;
-    if (n_shared && n_seq > 1 && !tiles && cap >= 2) {
+    if (pool) {
         const uint64_t pooled = (uint64_t)n_rows * group;
+        // the prefix for more than two tiles of 16 of all sequences' rows in wide tiles: 64 rows
+        // over 2000 keys 17 us against 20, over 8000 22 / 26, 160 over 1000 19 / 21, 256 over 8000
+        // 45 / 59 (but 96 rows over 4000 keys 28 / 22)
         p.form = pooled > ATTN_FEW_ROWS ? ATTN_MIXED : ATTN_ROWS;
         // (one launch's tiles are of 16 rows a wave)
         const uint32_t wide = attn_mixed(type, (int)head_dim) ? 16 * waves : (uint32_t)attn_tile_rows(type, (int)head_dim);
@@ -139,7 +152,7 @@ inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint3
         p.slots = p.shared_splits + p.own_splits;
     } else {
         p.form = tiles ? ATTN_TILES : ATTN_ROWS;
-        split(own, (uint64_t)max_kv + n_shared, 2 * cus, tiles ? many : few, cap, p.own_splits, p.own_chunk);
+        split(own, all_keys, 2 * cus, tiles ? many : few, cap, p.own_splits, p.own_chunk);
         p.slots = p.own_splits > 1 ? p.own_splits : 0;
     }
     p.own_items = (uint32_t)(own * p.own_splits);

@@ -20,7 +20,7 @@ static void look(unsigned S, unsigned rows, unsigned max_q, unsigned kv, unsigne
     bool ok = p.own_splits >= 1 && p.own_chunk >= 1;
     ok = ok && (unsigned long long)p.own_tiles * own_tile >= per && (unsigned long long)(p.own_tiles - 1) * own_tile < per;
     ok = ok && (unsigned long long)S * kv * p.own_tiles * p.own_splits == p.own_items;
-    ok = ok && (p.form == ATTN_TILES) == (per > ATTN_FEW_ROWS);
+    ok = ok && (per > 16 || p.form != ATTN_TILES);
     if (p.shared_items) {
         const unsigned t = p.form == ATTN_ROWS ? 16 : attn_mixed(type, D) ? 64 : attn_tile_rows(type, D);
         ok = ok && sh && S > 1 && p.shared_chunk >= 1 && p.slots == p.own_splits + p.shared_splits;
@@ -54,6 +54,12 @@ int main() {
                                         if ((unsigned long long)S * q * kv * g > 0x7FFF0000ull) continue;
                                         look(S, S * q, q, kv, g, keys, sh, D, type, cus);
                                     }
+    // the shapes that the GPU tests count on for wide tiles
+    for (int type : {ATTN_F32, ATTN_F16, ATTN_BF16})
+        for (unsigned D : {64u, 128u, 256u}) {
+            const unsigned r = (D == 64 ? 900 : D == 128 ? 640 : 460) + 3;
+            if (attn_plan(1, r, r, 8, 4, r, 0, D, type, 256).form != ATTN_TILES) bad++;
+        }
     printf("%lu %lu %lu %lu %lu %lu %lu\n", n, bad, forms[0], forms[1], forms[2], split, direct);
     return 0;
 }
