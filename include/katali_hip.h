@@ -166,7 +166,8 @@ int katali_hip_rmsnorm_matvec_f32(const float *x_dev, const float *delta_dev, fl
  * the packed rows q_start[s] .. q_start[s+1]-1 and kv_len[s] keys, the rows'
  * own among them: its rows are its newest positions, packed row
  * q_start[s+1]-1 stands at position kv_len[s]-1. q_start NULL: one row per
- * sequence, row s (n_rows == n_seq, max_q == 1). Rows before q_start[0], from
+ * sequence, row s (n_rows == n_seq, max_q == 1). q_start does not decrease, a
+ * kv_len above max_kv counts as max_kv. Rows before q_start[0], from
  * q_start[n_seq] on and past a sequence's first max_q are left as they were.
  * Caches: key j of sequence s and key head h at s * kv_seq_stride + j *
  * kv_row_stride + h * kv_head_stride values, head_dim values on end, k and v

@@ -60,6 +60,35 @@ def attn(c):
     return out
 
 
+def attn_wide(c):
+    """attn() for many rows: one matrix of scores for each sequence and head."""
+    H, KV, D = c["n_head"], c["n_kv"], c["D"]
+    out = np.full((c["n_rows"], H, D), np.nan)
+    for s in range(c["n_seq"]):
+        n, row = int(c["nq"][s]), int(c["q_start"][s])
+        if not n:
+            continue
+        pos, lo, hi = (np.asarray(x)[:, None] for x in zip(*[row_range(c, s, t, row + t) for t in range(n)]))
+        for g in range(KV):
+            k, v = c["k"][s, :int(c["kv_len"][s]), g], c["v"][s, :int(c["kv_len"][s]), g]
+            if c["n_shared"]:
+                k, v = np.concatenate([c["pk"][:, g], k]), np.concatenate([c["pv"][:, g], v])
+            j = np.arange(len(k))
+            seen = (j >= lo) & (j < hi)
+            for h in range(g * (H // KV), (g + 1) * (H // KV)):
+                x = c["scale"] * (c["q"][row:row + n, h].astype(np.float64) @ k.T)
+                if c["softcap"]:
+                    x = c["softcap"] * np.tanh(x / c["softcap"])
+                if c["slopes"] is not None:
+                    x = x - float(c["slopes"][h]) * np.abs(pos - j)
+                x = np.where(seen, x, -np.inf)
+                top = x.max(axis=1, keepdims=True)
+                p = np.exp(x - np.where(np.isfinite(top), top, 0.0))
+                total = p.sum(axis=1, keepdims=True)
+                out[row:row + n, h] = (p / np.where(total > 0, total, 1.0)) @ v
+    return out
+
+
 def make(rng, n_seq, nq, kv_len, max_kv, n_head, n_kv, D, t, causal=True, softcap=0.0, alibi=False, prefix=None,
          docs=None, n_shared=0, lead=0, tail=0, std=1.3, max_q=None):
     """A random call: `lead` and `tail` packed rows that belong to no sequence."""

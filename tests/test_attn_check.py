@@ -145,3 +145,13 @@ def test_oracle_bf16_rounds_to_nearest_even():
     assert val[0] == 1.0 and val[1] == 1.0 and val[2] == 1.015625 and val[3] == -1.0078125
     half = np.abs(val[:4] - x[:4]) <= 2.0 ** -8 * np.abs(x[:4])
     assert half.all() and raw.dtype == np.uint16
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(softcap=20.0), dict(alibi=True), dict(n_shared=13), dict(causal=False)])
+def test_the_two_forms_of_the_oracle_agree(kw):
+    import attn_oracle as O
+    rng = np.random.default_rng(3)
+    c = O.make(rng, 3, [5, 0, 9], [7, 4, 30], 30, 4, 2, 64, K.F16, prefix=[0, 3, 25], lead=1,
+               docs=lambda c: (rng.integers(0, 12, c["n_rows"]), rng.integers(0, 40, c["n_rows"])), **kw)
+    a, b = O.attn(c), O.attn_wide(c)
+    assert np.array_equal(np.isnan(a), np.isnan(b)) and np.nanmax(np.abs(a - b)) < 1e-12

@@ -115,6 +115,17 @@ def test_ragged_rows(hip, t):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("rows", [1, 50])
+@pytest.mark.parametrize("shared", [0, 70])
+def test_no_own_keys(hip, t, rows, shared):
+    """Caches of no rows: zeros, or the shared keys alone."""
+    rng = np.random.default_rng(22)
+    c = O.make(rng, 3, [rows] * 3, [0, 0, 0], 0, 4, 2, 64, t, n_shared=shared, causal=False)
+    check(hip, c)
+    check(hip, {**c, "causal": True})
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
 def test_not_causal(hip, t):
     rng = np.random.default_rng(4)
     check(hip, O.make(rng, 2, [37, 50], [100, 50], 100, 4, 2, 128, t, causal=False, alibi=True))
@@ -207,6 +218,37 @@ def test_shared_masks(hip, t):
     check(hip, O.make(rng, 4, [2, 0, 1, 2], [30, 5, 1, 2], 30, 6, 2, 64, t, n_shared=111, docs=documents))
     check(hip, O.make(rng, 4, [2, 0, 1, 2], [30, 5, 1, 2], 30, 6, 2, 64, t, n_shared=111, softcap=20.0, std=4.0,
                       prefix=[0, 50, 120, 200], lead=2, tail=1))
+
+
+# rows x keys from which tiles of 64 rows and more are taken (attn_plan), by
+# head width: 8 key heads of 4 query heads, one sequence, 256 CUs
+WIDE = {64: 900, 128: 640, 256: 460}
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("how", ["bare", "masks", "prefix", "unseen"])
+def test_wide_tiles(hip, t, D, how):
+    rng = np.random.default_rng(D)
+    n = WIDE[D] + 3
+    if how == "bare":
+        c = O.make(rng, 2, [n, n // 3], [n + 17, n // 2], n + 17, 32, 8, D, t, lead=1, tail=2)
+    elif how == "masks":
+        c = O.make(rng, 2, [n, n // 2], [n, n], n, 32, 8, D, t, docs=documents, alibi=True, softcap=30.0, std=3.0)
+    elif how == "prefix":   # a shared prefix walked ahead of own keys, seen from both sides beyond its end
+        c = O.make(rng, 2, [n, 5], [n, 70], n, 32, 8, D, t, n_shared=77, prefix=[150, 90], alibi=True)
+    else:                   # the last rows' key and what lies behind the end
+        c = O.make(rng, 1, [n], [n], n + 9, 32, 8, D, t)
+        for name in ("k", "v"):
+            c[name][0, n - 2:] = np.nan
+            c[name + "_raw"] = O.to_cache(c[name], t)[0]
+    print(f"[attn] wide {NAMES[t]} {how} rows={c['nq'].tolist()} keys={c['kv_len'].tolist()} of {D}", flush=True)
+    fine = {**c, "k": np.nan_to_num(c["k"]), "v": np.nan_to_num(c["v"])}
+    want, got = O.attn_wide(fine), O.run(hip, c)
+    if how == "unseen":
+        assert np.isnan(got[n - 2:]).all()
+        got[n - 2:], want[n - 2:] = 777.0, np.nan
+    O.compare(c, got, want)
 
 
 def test_long_cache_passes_32_bits(hip):
