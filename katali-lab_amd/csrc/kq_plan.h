@@ -132,8 +132,19 @@ inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint3
     auto few_for_cus = [&](uint64_t heads_rows, uint64_t n, uint64_t keys, uint64_t per_cu) {
         return cover(heads_rows, 16) * n * (keys ? keys : 1) <= per_cu * 128 / head_dim * cus;
     };
+    // Workgroups for tiles of 16 rows: two for each CU; with 16-bit caches one where that fills the CUs
+    // by 7/8 and 256-wide heads leave room for one only (3 tokens over 1600 keys of 8 heads 24 us
+    // with two, 17 with one; 60 rows over 1000 28 / 22) or one part for each item is that already
+    // (60 tokens over up to 9000 keys of 4 x 128 160 / 155 us; fp32 32 over 2000 of 8 x 128 62 / 67).
+    auto rows_want = [&](uint64_t items) {
+        const uint64_t n = cus / (items ? items : 1);
+        return !f32 && n * items * 8 >= 7ull * cus && (head_dim == 256 || n == 1) ? cus : 2 * cus;
+    };
     const uint64_t all_keys = (uint64_t)max_kv + n_shared;
-    const bool pool = n_shared && n_seq > 1 && per_seq <= ATTN_FEW_ROWS && cap >= 2;
+    // keys over which four waves take as long as a join
+    const uint64_t brief = (f32 ? 128 : 384) * 128 / head_dim;
+    // (over so few keys a shared prefix is walked by each sequence: 40 over 100 + 100 keys 11 us against 15)
+    const bool pool = n_shared && n_seq > 1 && per_seq <= ATTN_FEW_ROWS && cap >= 2 && all_keys > brief;
     const bool tiles = !pool && per_seq > 16 && !few_for_cus(per_seq, (uint64_t)n_seq * n_kv, all_keys, f32 ? 1400 : 3000);
     p.own_tiles = (uint32_t)cover(per_seq, tiles ? attn_tile_rows(type, (int)head_dim) : 16);
     const uint64_t own = (uint64_t)p.own_tiles * n_seq * n_kv;
@@ -148,11 +159,16 @@ inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint3
         p.shared_tiles = (uint32_t)cover(pooled, p.form == ATTN_MIXED ? wide : 16);
         split((uint64_t)n_kv * p.shared_tiles, n_shared, 2 * cus, p.form == ATTN_MIXED ? many : few, cap / 2,
               p.shared_splits, p.shared_chunk);
-        split(own, max_kv, 2 * cus, few, cap - p.shared_splits, p.own_splits, p.own_chunk);
+        split(own, max_kv, attn_mixed(type, (int)head_dim) ? 2 * cus : rows_want(own), few, cap - p.shared_splits, p.own_splits, p.own_chunk);
         p.slots = p.shared_splits + p.own_splits;
     } else {
         p.form = tiles ? ATTN_TILES : ATTN_ROWS;
-        split(own, all_keys, 2 * cus, tiles ? many : few, cap, p.own_splits, p.own_chunk);
+        split(own, all_keys, tiles ? 2 * cus : rows_want(own), tiles ? many : few, cap, p.own_splits, p.own_chunk);
+        // one part and no join where parts save less than the join costs, its price taken to grow with the
+        // rows to be joined: of 8 x 128 fp16, 1 token over 300 keys 10.6 us with parts, 9.1 without (560: 10.6 / 11.7),
+        // 20 over 1000 19.6 / 18.5, 32 over 600 19.7 / 17.4; fp32 1 over 130 10.3 / 10.0 (200: 10.4 / 11.4)
+        if (!tiles && all_keys * (p.own_splits - 1) * 8 * cus <= brief * p.own_splits * 3 * (2 * cus + 8 * own))
+            split(own, all_keys, 1, few, 1, p.own_splits, p.own_chunk);
         p.slots = p.own_splits > 1 ? p.own_splits : 0;
     }
     p.own_items = (uint32_t)(own * p.own_splits);

@@ -54,11 +54,15 @@ int main() {
                                         if ((unsigned long long)S * q * kv * g > 0x7FFF0000ull) continue;
                                         look(S, S * q, q, kv, g, keys, sh, D, type, cus);
                                     }
-    // the shapes that the GPU tests count on for wide tiles
+    // the shapes that the GPU tests count on: keys in parts, a prefix walked by all rows together, wide tiles
     for (int type : {ATTN_F32, ATTN_F16, ATTN_BF16})
         for (unsigned D : {64u, 128u, 256u}) {
             const unsigned r = (D == 64 ? 900 : D == 128 ? 640 : 460) + 3;
             if (attn_plan(1, r, r, 8, 4, r, 0, D, type, 256).form != ATTN_TILES) bad++;
+            if (attn_plan(4, 3, 1, 2, 4, 1900, 0, D, type, 256).own_splits < 2) bad++;
+            if (attn_plan(4, 19, 9, 2, 7, 1900, 0, D, type, 256).own_splits < 2) bad++;
+            const AttnPlan few = attn_plan(2, 1, 1, 2, 4, 300, 777, D, type, 256), many = attn_plan(9, 24, 3, 2, 4, 300, 790, D, type, 256);
+            if (few.form != ATTN_ROWS || !few.shared_items || many.form != ATTN_MIXED) bad++;
         }
     printf("%lu %lu %lu %lu %lu %lu %lu\n", n, bad, forms[0], forms[1], forms[2], split, direct);
     return 0;

@@ -220,6 +220,42 @@ def test_shared_masks(hip, t):
                       prefix=[0, 50, 120, 200], lead=2, tail=1))
 
 
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("how", ["bare", "masks", "unseen"])
+def test_parts_of_keys(hip, t, D, how):
+    """Keys in parts whose results are joined: sequences that fill all parts, some,
+    one and none, rows that see keys of one part only, one row and several tiles of rows."""
+    rng = np.random.default_rng(D)
+    masks = dict(docs=documents, alibi=True, softcap=30.0, std=3.0, prefix=[0, 1500, 9, 3]) if how == "masks" else {}
+    for rows, n_head in ((1, 8), (9, 14)):
+        c = O.make(rng, 4, [rows, rows, 1, 0], [1900, 1300, 33, 0], 1900, n_head, 2, D, t, **masks)
+        want = O.attn(c)
+        if how == "unseen":   # keys behind each sequence's end
+            for s in range(4):
+                for name in ("k", "v"):
+                    c[name][s, c["kv_len"][s]:] = np.inf
+            for name in ("k", "v"):
+                c[name + "_raw"] = O.to_cache(c[name], t)[0]
+        print(f"[attn] parts {NAMES[t]} {how} rows={rows} of {D}", flush=True)
+        O.compare(c, O.run(hip, c), want)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("how", ["bare", "cap", "masks"])
+@pytest.mark.parametrize("n_seq,rows,shared", [(2, 1, 777), (3, 1, 1001), (9, 3, 790), (21, 2, 1600)])
+def test_long_shared_prefix(hip, t, D, how, n_seq, rows, shared):
+    """Shared keys enough that the rows of all sequences walk them together:
+    one tile of rows to several, own keys from none to many."""
+    rng = np.random.default_rng(n_seq + shared)
+    nk = [300] + [int(rng.integers(rows, 300)) for _ in range(n_seq - 1)]
+    nk[-1] = 0
+    nq = [rows] * (n_seq - 1) + [0]
+    masks = dict(docs=documents, alibi=True, prefix=[900] * n_seq) if how == "masks" else {}
+    check(hip, O.make(rng, n_seq, nq, nk, 300, 8, 2, D, t, n_shared=shared, softcap=20.0 if how == "cap" else 0.0, **masks))
+
+
 # rows x keys from which tiles of 64 rows and more are taken (attn_plan), by
 # head width: 8 key heads of 4 query heads, one sequence, 256 CUs
 WIDE = {64: 900, 128: 640, 256: 460}
