@@ -141,6 +141,19 @@ inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint3
         return !f32 && n * items * 8 >= 7ull * cus && (head_dim == 256 || n == 1) ? cus : 2 * cus;
     };
     const uint64_t all_keys = (uint64_t)max_kv + n_shared;
+    // Workgroups for wide tiles, of which a CU holds two: two for each CU. Tiles that fill the CUs once
+    // and a part of them again are parted for four, else the second of a CU is alone with its keys for
+    // half the time, where the join is worth it: with fp32 up to 7/4 of the CUs (24 heads of 64, 1000 rows
+    // over 1000 keys, 376 tiles, 55 / 46 us; 528 rows over 2028, 264 tiles, 105 / 75), with 16 bits up to 3/2
+    // and from 1500 keys on (fp16, 264 tiles of 128: 1056 rows over 1056 keys 53 / 56, over 2556 130 / 105,
+    // over 5000 250 / 186). Of bf16 256 and fp32 128 a CU holds one: one for each CU where that fills them by
+    // 7/8 (1000 rows of 8 heads over 2 of bf16 256, 1000 keys 62 / 46; 4000 115 / 96; fp32 128 46 / 34 and 101 / 93).
+    auto tiles_want = [&](uint64_t items) {
+        const bool alone = (f32 && head_dim == 128) || (type == ATTN_BF16 && head_dim == 256);
+        const uint64_t n = cus / (items ? items : 1);
+        if (alone) return n * items * 8 >= 7ull * cus ? cus : 2 * cus;
+        return items > cus && (f32 ? items * 4 <= 7ull * cus : items * 2 <= 3ull * cus && all_keys >= 1500) ? 4 * cus : 2 * cus;
+    };
     // keys over which four waves take as long as a join
     const uint64_t brief = (f32 ? 128 : 384) * 128 / head_dim;
     // (over so few keys a shared prefix is walked by each sequence: 40 over 100 + 100 keys 11 us against 15)
@@ -157,13 +170,15 @@ inline AttnPlan attn_plan(uint32_t n_seq, uint32_t n_rows, uint32_t max_q, uint3
         // (one launch's tiles are of 16 rows a wave)
         const uint32_t wide = attn_mixed(type, (int)head_dim) ? 16 * waves : (uint32_t)attn_tile_rows(type, (int)head_dim);
         p.shared_tiles = (uint32_t)cover(pooled, p.form == ATTN_MIXED ? wide : 16);
-        split((uint64_t)n_kv * p.shared_tiles, n_shared, 2 * cus, p.form == ATTN_MIXED ? many : few, cap / 2,
-              p.shared_splits, p.shared_chunk);
-        split(own, max_kv, attn_mixed(type, (int)head_dim) ? 2 * cus : rows_want(own), few, cap - p.shared_splits, p.own_splits, p.own_chunk);
+        const uint64_t shared = (uint64_t)n_kv * p.shared_tiles;
+        const bool apart = !attn_mixed(type, (int)head_dim);   // two launches
+        split(shared, n_shared, apart && p.form == ATTN_MIXED ? tiles_want(shared) : 2 * cus,
+              p.form == ATTN_MIXED ? many : few, cap / 2, p.shared_splits, p.shared_chunk);
+        split(own, max_kv, apart ? rows_want(own) : 2 * cus, few, cap - p.shared_splits, p.own_splits, p.own_chunk);
         p.slots = p.shared_splits + p.own_splits;
     } else {
         p.form = tiles ? ATTN_TILES : ATTN_ROWS;
-        split(own, all_keys, tiles ? 2 * cus : rows_want(own), tiles ? many : few, cap, p.own_splits, p.own_chunk);
+        split(own, all_keys, tiles ? tiles_want(own) : rows_want(own), tiles ? many : few, cap, p.own_splits, p.own_chunk);
         // one part and no join where parts save less than the join costs, its price taken to grow with the
         // rows to be joined: of 8 x 128 fp16, 1 token over 300 keys 10.6 us with parts, 9.1 without (560: 10.6 / 11.7),
         // 20 over 1000 19.6 / 18.5, 32 over 600 19.7 / 17.4; fp32 1 over 130 10.3 / 10.0 (200: 10.4 / 11.4)
