@@ -1185,20 +1185,18 @@ __global__ void __launch_bounds__(64 * ROWS_WAVES, 2) k_attn_mixed(const AttnArg
     else attn_rows_item<TY, D, W>(a, it, lds);
 }
 
-// The partial sums of a row, joined: SW waves per (row, head), each every
-// SW-th slot, eight slots' loads in flight. 2.5 us where little is to be joined
-// (a launch), 4.6 us for 64 slots of 32 rows (one wave a row, one slot after
-// another: 12 us).
-template <int D, int SW>
+// The partial sums of a row, joined. Many slots: a workgroup per (row, head),
+// its four waves each every fourth slot, eight slots' loads in flight (64
+// slots of 32 rows 4.6 us; one wave a row, one slot after another: 12 us).
+template <int D>
 __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
-    constexpr int E = D / 64, U = 8;
-    __shared__ float part[SW > 1 ? SW : 1][SW > 1 ? D : 1];
+    constexpr int E = D / 64, U = 8, SW = 4;
+    __shared__ float part[SW][D];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t per = 4 / SW, blocks = (a.n_head + per - 1) / per;
-    const uint32_t head = blockIdx.x % blocks * per + wave / SW;
-    const uint32_t id = blockIdx.x / blocks, seq = id / a.max_q, t = id % a.max_q;
+    const uint32_t head = blockIdx.x % a.n_head;
+    const uint32_t id = blockIdx.x / a.n_head, seq = id / a.max_q, t = id % a.max_q;
     const SeqRows sr = seq_rows(a, seq);
-    if (head >= a.n_head || (int32_t)t >= sr.last - sr.first) return;
+    if ((int32_t)t >= sr.last - sr.first) return;
     const uint64_t rh = (uint64_t)(uint32_t)(sr.first + (int32_t)t) * a.n_head + head;
     float2 ml = make_float2(NEG_INF, 0.0f);
     if ((uint32_t)lane < a.slots) ml = a.ml[rh * a.slots + lane];
@@ -1212,7 +1210,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
 #pragma unroll
     for (int e = 0; e < E; e++) x[e] = 0.0f;
     const float *p = a.acc + rh * a.slots * D + lane;
-    for (uint32_t k0 = wave % SW; k0 < a.slots; k0 += SW * U) {
+    for (uint32_t k0 = wave; k0 < a.slots; k0 += SW * U) {
         float v[U][E];
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -1227,18 +1225,55 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
             for (int e = 0; e < E; e++) x[e] = wk == 0.0f ? x[e] : fmaf(v[u][e], wk, x[e]);
         }
     }
-    if constexpr (SW > 1) {
 #pragma unroll
-        for (int e = 0; e < E; e++) part[wave][lane + 64 * e] = x[e];
-        __syncthreads();
-        if (wave) return;
+    for (int e = 0; e < E; e++) part[wave][lane + 64 * e] = x[e];
+    __syncthreads();
+    if (wave) return;
 #pragma unroll
-        for (int e = 0; e < E; e++)
+    for (int e = 0; e < E; e++) {
 #pragma unroll
-            for (int k = 1; k < SW; k++) x[e] += part[k][lane + 64 * e];
+        for (int k = 1; k < SW; k++) x[e] += part[k][lane + 64 * e];
+        a.out[rh * D + lane + 64 * e] = x[e] * f0;
     }
+}
+
+// Up to U slots, four or eight: four values a lane, D / 4 lanes per (row,
+// head), each with all slots' maxima and sums, all loads at once: 24 heads of
+// 64, 1000 rows, two slots, 5.2 us (a wave for each of the rows, a value a
+// lane, 9.6), a launch (2.5) where little is to be joined. Only 300 rows of 32
+// heads of 64 with six slots lost by it, 44 us to 47 the whole call.
+constexpr uint32_t JOIN_FEW = 8;
+template <int D, int U>
+__global__ void __launch_bounds__(256) k_attn_join_few(const AttnArgs a) {
+    constexpr uint32_t L = D / 4;
+    const uint32_t at = blockIdx.x * (256 / L) + threadIdx.x / L, i = threadIdx.x % L;
+    const uint32_t head = at % a.n_head, id = at / a.n_head, seq = id / a.max_q, t = id % a.max_q;
+    if (seq >= a.n_seq) return;
+    const SeqRows sr = seq_rows(a, seq);
+    if ((int32_t)t >= sr.last - sr.first) return;
+    const uint64_t rh = (uint64_t)(uint32_t)(sr.first + (int32_t)t) * a.n_head + head;
+    const float2 *q = a.ml + rh * a.slots;
+    const float4 *p = (const float4 *)(a.acc + rh * a.slots * D) + i;
+    float2 ml[U];
+    float4 v[U];
 #pragma unroll
-    for (int e = 0; e < E; e++) a.out[rh * D + lane + 64 * e] = x[e] * f0;
+    for (uint32_t u = 0; u < U; u++) ml[u] = q[min(u, a.slots - 1)];
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++) v[u] = p[min(u, a.slots - 1) * L];
+    float m = NEG_INF, l = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++) m = fmaxf(m, ml[u].x);
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++) {
+        const float w = u >= a.slots || ml[u].y == 0.0f ? 0.0f : exp2_hw(ml[u].x - m);
+        l = fmaf(ml[u].y, w, l);
+        const float y[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+        // a slot that weighs nothing may hold anything
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = w == 0.0f ? x[e] : fmaf(y[e], w, x[e]);
+    }
+    const float f0 = l == 0.0f ? 0.0f : 1.0f / l;
+    ((float4 *)(a.out + rh * D))[i] = make_float4(x[0] * f0, x[1] * f0, x[2] * f0, x[3] * f0);
 }
 
 template <int TY, int D>
@@ -1264,8 +1299,9 @@ static hipError_t attn_run(const AttnArgs &a, const AttnPlan &p, hipStream_t s) 
     if (e != hipSuccess || !a.slots) return e;
     // four waves a row where many slots meet
     const uint32_t n = a.n_seq * a.max_q;
-    if (a.slots > 8) hipLaunchKernelGGL((k_attn_join<D, 4>), dim3(n * a.n_head), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_attn_join<D, 1>), dim3(n * ((a.n_head + 3) / 4)), dim3(256), 0, s, a);
+    if (a.slots > JOIN_FEW) hipLaunchKernelGGL((k_attn_join<D>), dim3(n * a.n_head), dim3(256), 0, s, a);
+    else if (a.slots > 4) hipLaunchKernelGGL((k_attn_join_few<D, 8>), dim3((n * a.n_head + 1024 / D - 1) / (1024 / D)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_join_few<D, 4>), dim3((n * a.n_head + 1024 / D - 1) / (1024 / D)), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

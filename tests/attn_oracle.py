@@ -82,7 +82,7 @@ def attn_wide(c):
                 if c["slopes"] is not None:
                     x = x - float(c["slopes"][h]) * np.abs(pos - j)
                 x = np.where(seen, x, -np.inf)
-                top = x.max(axis=1, keepdims=True)
+                top = x.max(axis=1, keepdims=True, initial=-np.inf)
                 p = np.exp(x - np.where(np.isfinite(top), top, 0.0))
                 total = p.sum(axis=1, keepdims=True)
                 out[row:row + n, h] = (p / np.where(total > 0, total, 1.0)) @ v
