@@ -623,7 +623,7 @@ __device__ __forceinline__ Item make_item(const AttnArgs &a, uint32_t id) {
     return it;
 }
 
-// A row's result: the output itself, or one of the partial sums that k_attn_join joins.
+// A row's result: the output itself, or one of the partial sums that k_attn_join and k_attn_join_few join.
 __device__ __forceinline__ uint64_t row_head(const AttnArgs &a, const Row &r) {
     return (uint64_t)(uint32_t)r.row * a.n_head + r.head;
 }
@@ -1242,7 +1242,6 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
 // 64, 1000 rows, two slots, 5.2 us (a wave for each of the rows, a value a
 // lane, 9.6), a launch (2.5) where little is to be joined. Only 300 rows of 32
 // heads of 64 with six slots lost by it, 44 us to 47 the whole call.
-constexpr uint32_t JOIN_FEW = 8;
 template <int D, int U>
 __global__ void __launch_bounds__(256) k_attn_join_few(const AttnArgs a) {
     constexpr uint32_t L = D / 4;
@@ -1299,9 +1298,10 @@ static hipError_t attn_run(const AttnArgs &a, const AttnPlan &p, hipStream_t s) 
     if (e != hipSuccess || !a.slots) return e;
     // four waves a row where many slots meet
     const uint32_t n = a.n_seq * a.max_q;
-    if (a.slots > JOIN_FEW) hipLaunchKernelGGL((k_attn_join<D>), dim3(n * a.n_head), dim3(256), 0, s, a);
-    else if (a.slots > 4) hipLaunchKernelGGL((k_attn_join_few<D, 8>), dim3((n * a.n_head + 1024 / D - 1) / (1024 / D)), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_attn_join_few<D, 4>), dim3((n * a.n_head + 1024 / D - 1) / (1024 / D)), dim3(256), 0, s, a);
+    const uint32_t few = (n * a.n_head + 1024 / D - 1) / (1024 / D);
+    if (a.slots > 8) hipLaunchKernelGGL((k_attn_join<D>), dim3(n * a.n_head), dim3(256), 0, s, a);
+    else if (a.slots > 4) hipLaunchKernelGGL((k_attn_join_few<D, 8>), dim3(few), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_join_few<D, 4>), dim3(few), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

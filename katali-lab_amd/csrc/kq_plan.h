@@ -75,8 +75,8 @@ inline bool down_plan(bool q6, uint32_t hidden, uint32_t ffn, uint32_t n_slots, 
 // How an attention call's rows and keys are spread over workgroups. The rows
 // of one key head of a sequence (query rows x the heads that share the key
 // head) make tiles: of 16 where they are few (the waves of a workgroup share
-// the rows and divide the keys), else of 128, 16 or 32 to a wave, which walk
-// the same keys together. Keys are split where the tiles alone would leave
+// the rows and divide the keys), else of 64 or 128, 16 or 32 to a wave, which
+// walk the same keys together. Keys are split where the tiles alone would leave
 // CUs idle; the parts' sums meet in `slots` partial results of each row
 // (0: one part, written as the output). A shared prefix is either an item of
 // its own for the rows of all sequences together (shared_tiles > 0), or
@@ -91,7 +91,7 @@ struct AttnPlan {
 constexpr uint32_t ATTN_MAX_SLOTS = 64;
 constexpr uint64_t ATTN_SCRATCH = 64ull << 20;   // partial results: head_dim sums, a maximum and a sum each
 constexpr uint32_t ATTN_FEW_ROWS = 32;           // rows of a key head: up to here a sequence's rows are pooled over a shared
-                                                 // prefix, beyond it the pool takes wide tiles
+                                                 // prefix, and a pool of more takes wide tiles
 constexpr int ATTN_F32 = 0, ATTN_F16 = 1, ATTN_BF16 = 30;   // cache types (ggml ids)
 // Rows of a workgroup's tile: 16 or 32 for each of four or eight waves, by what registers and LDS hold.
 constexpr int attn_tile_rows(int type, int head_dim) {
